@@ -117,6 +117,60 @@ class PeerReduceParams(ctypes.Structure):
                 ("max_polls", ctypes.c_uint32), ("flags", ctypes.c_uint32), ("status", c_ptr)]
 
 
+class ScanParams(ctypes.Structure):
+    _fields_ = [
+        ("dtype", c_i32), ("dt_dtype", c_i32), ("init_dtype", c_i32), ("dt_softplus", c_i32),
+        ("batch", c_i64), ("seqlen", c_i64), ("nheads", c_i64), ("headdim", c_i64), ("ngroups", c_i64),
+        ("dstate", c_i64),
+        ("x", c_ptr), ("x_batch_stride", c_i64), ("x_seq_stride", c_i64), ("x_head_stride", c_i64),
+        ("x_dim_stride", c_i64),
+        ("dt", c_ptr), ("dt_batch_stride", c_i64), ("dt_seq_stride", c_i64), ("dt_head_stride", c_i64),
+        ("B", c_ptr), ("B_batch_stride", c_i64), ("B_seq_stride", c_i64), ("B_group_stride", c_i64),
+        ("B_state_stride", c_i64),
+        ("C", c_ptr), ("C_batch_stride", c_i64), ("C_seq_stride", c_i64), ("C_group_stride", c_i64),
+        ("C_state_stride", c_i64),
+        ("A", c_ptr), ("D", c_ptr), ("dt_bias", c_ptr), ("cu_seqlens", c_ptr),
+        ("num_seqs", c_i64), ("max_seqlen", c_i64),
+        ("initial_states", c_ptr), ("init_seq_stride", c_i64), ("init_head_stride", c_i64),
+        ("y", c_ptr), ("y_batch_stride", c_i64), ("y_seq_stride", c_i64), ("y_head_stride", c_i64),
+        ("final_states", c_ptr), ("final_seq_stride", c_i64), ("final_head_stride", c_i64),
+        ("workspace", c_ptr), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class ScanUpdateParams(ctypes.Structure):
+    _fields_ = [
+        ("dtype", c_i32), ("dt_dtype", c_i32), ("state_dtype", c_i32), ("dt_softplus", c_i32),
+        ("batch", c_i64), ("nheads", c_i64), ("headdim", c_i64), ("ngroups", c_i64), ("dstate", c_i64),
+        ("state_rows", c_i64),
+        ("x", c_ptr), ("x_batch_stride", c_i64), ("x_head_stride", c_i64), ("x_dim_stride", c_i64),
+        ("dt", c_ptr), ("dt_batch_stride", c_i64), ("dt_head_stride", c_i64),
+        ("B", c_ptr), ("B_batch_stride", c_i64), ("B_group_stride", c_i64), ("B_state_stride", c_i64),
+        ("C", c_ptr), ("C_batch_stride", c_i64), ("C_group_stride", c_i64), ("C_state_stride", c_i64),
+        ("A", c_ptr), ("D", c_ptr), ("dt_bias", c_ptr),
+        ("state", c_ptr), ("state_row_stride", c_i64), ("state_head_stride", c_i64), ("state_dim_stride", c_i64),
+        ("state_indices", c_ptr), ("out_state_indices", c_ptr),
+        ("y", c_ptr), ("y_batch_stride", c_i64), ("y_head_stride", c_i64),
+    ]
+
+
+class GatedNormParams(ctypes.Structure):
+    _fields_ = [
+        ("dtype", c_i32), ("weight_dtype", c_i32), ("layer", c_i32), ("gate_first", c_i32),
+        ("rows", c_i64), ("dim", c_i64), ("group_size", c_i64), ("eps", ctypes.c_float), ("_pad0", c_i32),
+        ("x", c_ptr), ("x_row_stride", c_i64),
+        ("z", c_ptr), ("z_row_stride", c_i64),
+        ("weight", c_ptr), ("bias", c_ptr),
+        ("y", c_ptr), ("y_row_stride", c_i64),
+        ("mean", c_ptr), ("rstd", c_ptr),
+        ("dy", c_ptr), ("dy_row_stride", c_i64),
+        ("dx", c_ptr), ("dx_row_stride", c_i64),
+        ("dz", c_ptr), ("dz_row_stride", c_i64),
+        ("dweight", c_ptr), ("dbias", c_ptr),
+        ("workspace", c_ptr), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
 # cc1d_peer_reduce.flags
 PEER_FUSED = 0
 PEER_PUSH = 1
@@ -135,6 +189,12 @@ SIGNATURES = {
     "cc1d_update": (c_i32, [ctypes.POINTER(UpdateParams), c_ptr]),
     "cc1d_varlen_states": (c_i32, [ctypes.POINTER(VarlenParams), c_ptr]),
     "cc1d_inproj_conv_fwd": (c_i32, [ctypes.POINTER(InprojConvParams), c_ptr]),
+    "cc1d_scan_workspace_size": (c_i32, [ctypes.POINTER(ScanParams), ctypes.POINTER(ctypes.c_size_t)]),
+    "cc1d_scan": (c_i32, [ctypes.POINTER(ScanParams), c_ptr]),
+    "cc1d_scan_update": (c_i32, [ctypes.POINTER(ScanUpdateParams), c_ptr]),
+    "cc1d_gated_norm_fwd": (c_i32, [ctypes.POINTER(GatedNormParams), c_ptr]),
+    "cc1d_gated_norm_workspace_size": (c_i32, [ctypes.POINTER(GatedNormParams), ctypes.POINTER(ctypes.c_size_t)]),
+    "cc1d_gated_norm_bwd": (c_i32, [ctypes.POINTER(GatedNormParams), c_ptr]),
     "cc1d_device_status": (c_i32, [ctypes.POINTER(ctypes.c_uint)]),
     "cc1d_last_error": (ctypes.c_char_p, []),
     "cc1d_version": (ctypes.c_char_p, []),

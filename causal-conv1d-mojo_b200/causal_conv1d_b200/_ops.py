@@ -388,3 +388,194 @@ def _inproj_conv_fake(hidden, in_weight, conv_weight, conv_bias, initial_states,
 inproj_conv = torch.library.custom_op(
     "causal_conv1d_b200::inproj_conv", mutates_args=("out", "final_states_out"))(_inproj_conv_impl)
 inproj_conv.register_fake(_inproj_conv_fake)
+
+
+# ---- state space scan, its single-token step, gated norm ----
+#
+# Small calls of these are bound by the host, so outside of compilation the
+# public functions call the implementation below without going through the
+# dispatcher (`_pick`); a compiled program sees the custom op.
+
+
+def _pick(op, impl):
+    return op if torch.compiler.is_compiling() else impl
+
+
+def _scan_impl(
+    x: torch.Tensor,
+    dt: torch.Tensor,
+    A: torch.Tensor,
+    B: torch.Tensor,
+    C: torch.Tensor,
+    D: torch.Tensor | None,
+    dt_bias: torch.Tensor | None,
+    dt_softplus: bool,
+    initial_states: torch.Tensor | None,
+    cu_seqlens: torch.Tensor | None,
+    max_seqlen: int,
+    y: torch.Tensor,
+    final_states_out: torch.Tensor | None,
+) -> None:
+    """y (and final_states_out) = the scan of cc1d_scan; the workspace for sequences
+    that are split over their length is allocated here."""
+    _require_cuda(x, "state_space_scan")
+    lib = _lib.load()
+    batch, seqlen, H, P = x.shape
+    code = _DTYPE_CODE
+    init = initial_states
+    p = _lib.ScanParams(
+        code[x.dtype], code[dt.dtype], code[x.dtype] if init is None else code[init.dtype], 1 if dt_softplus else 0,
+        batch, seqlen, H, P, B.shape[2], B.shape[3],
+        x.data_ptr(), *x.stride(), dt.data_ptr(), *dt.stride(), B.data_ptr(), *B.stride(), C.data_ptr(), *C.stride(),
+        A.data_ptr(), _ptr(D), _ptr(dt_bias), _ptr(cu_seqlens),
+        0 if cu_seqlens is None else cu_seqlens.shape[0] - 1, max_seqlen,
+        _ptr(init), *((0, 0) if init is None else init.stride()[:2]),
+        y.data_ptr(), *y.stride()[:3],
+        _ptr(final_states_out), *((0, 0) if final_states_out is None else final_states_out.stride()[:2]))
+    with _on_device(x.device):
+        n = ctypes.c_size_t(0)
+        _lib.check(lib.cc1d_scan_workspace_size(ctypes.byref(p), ctypes.byref(n)), "cc1d_scan_workspace_size")
+        if n.value > 0:
+            ws = torch.empty(n.value, dtype=torch.uint8, device=x.device)
+            p.workspace, p.workspace_bytes = ws.data_ptr(), n.value
+        _lib.check(lib.cc1d_scan(ctypes.byref(p), _stream(x.device)), "cc1d_scan")
+
+
+def _scan_fake(x, dt, A, B, C, D, dt_bias, dt_softplus, initial_states, cu_seqlens, max_seqlen, y,
+               final_states_out) -> None:
+    return None
+
+
+_scan_op = torch.library.custom_op("causal_conv1d_b200::scan", mutates_args=("y", "final_states_out"))(_scan_impl)
+_scan_op.register_fake(_scan_fake)
+
+
+def scan(*args):
+    _pick(_scan_op, _scan_impl)(*args)
+
+
+def _scan_update_impl(
+    x: torch.Tensor,
+    state: torch.Tensor,
+    dt: torch.Tensor,
+    A: torch.Tensor,
+    B: torch.Tensor,
+    C: torch.Tensor,
+    D: torch.Tensor | None,
+    dt_bias: torch.Tensor | None,
+    dt_softplus: bool,
+    state_indices: torch.Tensor | None,
+    out_state_indices: torch.Tensor | None,
+    y: torch.Tensor,
+) -> None:
+    _require_cuda(x, "state_space_update")
+    lib = _lib.load()
+    batch, H, P = x.shape
+    code = _DTYPE_CODE
+    p = _lib.ScanUpdateParams(
+        code[x.dtype], code[dt.dtype], code[state.dtype], 1 if dt_softplus else 0,
+        batch, H, P, B.shape[1], B.shape[2], state.shape[0],
+        x.data_ptr(), *x.stride(), dt.data_ptr(), *dt.stride(), B.data_ptr(), *B.stride(), C.data_ptr(), *C.stride(),
+        A.data_ptr(), _ptr(D), _ptr(dt_bias), state.data_ptr(), *state.stride()[:3],
+        _ptr(state_indices), _ptr(out_state_indices), y.data_ptr(), *y.stride()[:2])
+    with _on_device(x.device):
+        _lib.check(lib.cc1d_scan_update(ctypes.byref(p), _stream(x.device)), "cc1d_scan_update")
+
+
+def _scan_update_fake(x, state, dt, A, B, C, D, dt_bias, dt_softplus, state_indices, out_state_indices, y) -> None:
+    return None
+
+
+_scan_update_op = torch.library.custom_op(
+    "causal_conv1d_b200::scan_update", mutates_args=("state", "y"))(_scan_update_impl)
+_scan_update_op.register_fake(_scan_update_fake)
+
+
+def scan_update(*args):
+    _pick(_scan_update_op, _scan_update_impl)(*args)
+
+
+def _norm_fwd_impl(
+    x: torch.Tensor,
+    z: torch.Tensor | None,
+    weight: torch.Tensor,
+    bias: torch.Tensor | None,
+    eps: float,
+    group_size: int,
+    layer: bool,
+    gate_first: bool,
+    y: torch.Tensor,
+    mean: torch.Tensor | None,
+    rstd: torch.Tensor | None,
+) -> None:
+    """x, z, y (rows, dim) with unit stride over dim; mean and rstd (rows, groups) fp32 or None."""
+    _require_cuda(x, "gated_norm_fn")
+    lib = _lib.load()
+    p = _lib.GatedNormParams(
+        _DTYPE_CODE[x.dtype], _DTYPE_CODE[weight.dtype], 1 if layer else 0, 1 if gate_first else 0,
+        x.shape[0], x.shape[1], group_size, eps, 0,
+        x.data_ptr(), x.stride(0), _ptr(z), 0 if z is None else z.stride(0), weight.data_ptr(), _ptr(bias),
+        y.data_ptr(), y.stride(0), _ptr(mean), _ptr(rstd))
+    with _on_device(x.device):
+        _lib.check(lib.cc1d_gated_norm_fwd(ctypes.byref(p), _stream(x.device)), "cc1d_gated_norm_fwd")
+
+
+def _norm_fwd_fake(x, z, weight, bias, eps, group_size, layer, gate_first, y, mean, rstd) -> None:
+    return None
+
+
+_norm_fwd_op = torch.library.custom_op(
+    "causal_conv1d_b200::gated_norm_fwd", mutates_args=("y", "mean", "rstd"))(_norm_fwd_impl)
+_norm_fwd_op.register_fake(_norm_fwd_fake)
+
+
+def norm_fwd(*args):
+    _pick(_norm_fwd_op, _norm_fwd_impl)(*args)
+
+
+def _norm_bwd_impl(
+    x: torch.Tensor,
+    z: torch.Tensor | None,
+    weight: torch.Tensor,
+    bias: torch.Tensor | None,
+    dy: torch.Tensor,
+    mean: torch.Tensor | None,
+    rstd: torch.Tensor,
+    eps: float,
+    group_size: int,
+    layer: bool,
+    gate_first: bool,
+    dx: torch.Tensor,
+    dz: torch.Tensor | None,
+    dweight: torch.Tensor,
+    dbias: torch.Tensor | None,
+) -> None:
+    _require_cuda(x, "gated_norm_fn")
+    lib = _lib.load()
+    p = _lib.GatedNormParams(
+        _DTYPE_CODE[x.dtype], _DTYPE_CODE[weight.dtype], 1 if layer else 0, 1 if gate_first else 0,
+        x.shape[0], x.shape[1], group_size, eps, 0,
+        x.data_ptr(), x.stride(0), _ptr(z), 0 if z is None else z.stride(0), weight.data_ptr(), _ptr(bias),
+        0, 0, _ptr(mean), rstd.data_ptr(), dy.data_ptr(), dy.stride(0), dx.data_ptr(), dx.stride(0),
+        _ptr(dz), 0 if dz is None else dz.stride(0), dweight.data_ptr(), _ptr(dbias))
+    with _on_device(x.device):
+        n = ctypes.c_size_t(0)
+        _lib.check(lib.cc1d_gated_norm_workspace_size(ctypes.byref(p), ctypes.byref(n)),
+                   "cc1d_gated_norm_workspace_size")
+        ws = torch.empty(n.value, dtype=torch.uint8, device=x.device)
+        p.workspace, p.workspace_bytes = ws.data_ptr(), n.value
+        _lib.check(lib.cc1d_gated_norm_bwd(ctypes.byref(p), _stream(x.device)), "cc1d_gated_norm_bwd")
+
+
+def _norm_bwd_fake(x, z, weight, bias, dy, mean, rstd, eps, group_size, layer, gate_first, dx, dz, dweight,
+                   dbias) -> None:
+    return None
+
+
+_norm_bwd_op = torch.library.custom_op(
+    "causal_conv1d_b200::gated_norm_bwd", mutates_args=("dx", "dz", "dweight", "dbias"))(_norm_bwd_impl)
+_norm_bwd_op.register_fake(_norm_bwd_fake)
+
+
+def norm_bwd(*args):
+    _pick(_norm_bwd_op, _norm_bwd_impl)(*args)

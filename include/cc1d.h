@@ -290,6 +290,135 @@ typedef struct cc1d_inproj_conv_params {
 
 CC1D_API int cc1d_inproj_conv_fwd(const cc1d_inproj_conv_params* params, void* stream);
 
+/*
+ * Selective state space scan over prompts: the step of a Mamba-2 style block
+ * that follows the causal conv.  Per sequence, head h (of group
+ * g = h / (nheads / ngroups)) and token t, with a (headdim, dstate) state S:
+ *   dt' = softplus(dt + dt_bias)   (softplus only with dt_softplus != 0)
+ *   S_t = exp(dt' * A[h]) * S_{t-1} + dt' * x_t (outer) B_t
+ *   y_t = S_t C_t + D[h] * x_t
+ * S starts from initial_states (or zeros); final_states (optional, fp32)
+ * receives the last S of each sequence.  The state is fp32 throughout.
+ *
+ * Sequences: without cu_seqlens the batch rows, seqlen tokens each.  With
+ * cu_seqlens (device, num_seqs + 1 non-decreasing entries; batch == 1) the
+ * token ranges [cu_seqlens[i], cu_seqlens[i+1]) of the one row; a range may
+ * be empty (its final state is its initial state), and tokens outside every
+ * range get y = 0.  max_seqlen (0: unknown) is an upper bound of the range
+ * lengths and only steers how work is split.
+ *
+ * x and y (batch, seqlen, nheads, headdim), B and C (batch, seqlen, ngroups,
+ * dstate) and dt (batch, seqlen, nheads) take any strides; y has unit stride
+ * over headdim.  initial_states and final_states (num_seqs, nheads, headdim,
+ * dstate) are contiguous over their last two dimensions.
+ *
+ * `workspace` (size from cc1d_scan_workspace_size) holds the partial states
+ * of sequences that are split over their length.
+ *
+ * No counterpart in the reference, which ends at the conv.
+ */
+typedef struct cc1d_scan_params {
+  int32_t dtype;          /* x, B, C, y */
+  int32_t dt_dtype;       /* dtype or CC1D_F32 */
+  int32_t init_dtype;     /* dtype or CC1D_F32 */
+  int32_t dt_softplus;
+  int64_t batch, seqlen, nheads, headdim, ngroups, dstate;  /* dstate <= 256 */
+  const void* x;          int64_t x_batch_stride, x_seq_stride, x_head_stride, x_dim_stride;
+  const void* dt;         int64_t dt_batch_stride, dt_seq_stride, dt_head_stride;
+  const void* B;          int64_t B_batch_stride, B_seq_stride, B_group_stride, B_state_stride;
+  const void* C;          int64_t C_batch_stride, C_seq_stride, C_group_stride, C_state_stride;
+  const float* A;         /* (nheads), contiguous */
+  const float* D;         /* (nheads), contiguous; NULL: 0 */
+  const float* dt_bias;   /* (nheads), contiguous; NULL: 0 */
+  const int32_t* cu_seqlens; /* NULL: none */
+  int64_t num_seqs, max_seqlen;
+  const void* initial_states; int64_t init_seq_stride, init_head_stride;  /* NULL: zeros */
+  void* y;                int64_t y_batch_stride, y_seq_stride, y_head_stride;
+  float* final_states;    int64_t final_seq_stride, final_head_stride;    /* NULL: not written */
+  void* workspace;        size_t workspace_bytes;
+} cc1d_scan_params;
+
+CC1D_API int cc1d_scan_workspace_size(const cc1d_scan_params* params, size_t* bytes);
+
+CC1D_API int cc1d_scan(const cc1d_scan_params* params, void* stream);
+
+/*
+ * The scan's step for single tokens, on a pool of states:
+ * state (state_rows, nheads, headdim, dstate), unit stride over dstate, in
+ * `dtype` or fp32 (the step itself is computed in fp32 either way).
+ * Batch row b reads state row state_indices[b] (b itself when NULL) and
+ * writes the new state to row out_state_indices[b] (the row it read when
+ * NULL).  A read index outside [0, state_rows) gives y[b] = 0 and writes no
+ * state; a write index outside it drops the new state.  No two batch rows
+ * may write one row, nor may one write a row that another reads.
+ * No counterpart in the reference.
+ */
+typedef struct cc1d_scan_update_params {
+  int32_t dtype;          /* x, B, C, y */
+  int32_t dt_dtype;       /* dtype or CC1D_F32 */
+  int32_t state_dtype;    /* dtype or CC1D_F32 */
+  int32_t dt_softplus;
+  int64_t batch, nheads, headdim, ngroups, dstate;  /* dstate <= 256 */
+  int64_t state_rows;
+  const void* x;          int64_t x_batch_stride, x_head_stride, x_dim_stride;
+  const void* dt;         int64_t dt_batch_stride, dt_head_stride;
+  const void* B;          int64_t B_batch_stride, B_group_stride, B_state_stride;
+  const void* C;          int64_t C_batch_stride, C_group_stride, C_state_stride;
+  const float* A;
+  const float* D;         /* NULL: 0 */
+  const float* dt_bias;   /* NULL: 0 */
+  void* state;            int64_t state_row_stride, state_head_stride, state_dim_stride;
+  const int32_t* state_indices;     /* NULL: row b */
+  const int32_t* out_state_indices; /* NULL: the row that was read */
+  void* y;                int64_t y_batch_stride, y_head_stride;  /* unit stride over headdim */
+} cc1d_scan_update_params;
+
+CC1D_API int cc1d_scan_update(const cc1d_scan_update_params* params, void* stream);
+
+/*
+ * Gated norm over groups of group_size adjacent columns of each row of
+ * x (rows, dim):
+ *   u = gate_first ? x * silu(z) : x            (z NULL: u = x)
+ *   n = (u - mean(u)) / sqrt(mean((u - mean(u))^2) + eps)   mean(u) taken as 0 unless layer != 0
+ *   y = n * weight + bias,  times silu(z) when gate_first == 0
+ * Every row pitch is free; columns have unit stride; weight and bias (dim)
+ * are contiguous, in `dtype` or fp32.  mean and rstd (rows, dim / group_size,
+ * fp32, contiguous; mean only with layer) are written for the backward when
+ * given.
+ *
+ * Backward: dx, dz and the sums over rows dweight and dbias (weight's
+ * dtype), from dy and the forward's mean and rstd.  Each block keeps its
+ * rows' share of the weight and bias gradients in registers and writes it to
+ * `workspace` (size from cc1d_gated_norm_workspace_size); a second kernel
+ * adds the shares in a fixed order, so results are bitwise reproducible.
+ * No counterpart in the reference.
+ */
+typedef struct cc1d_gated_norm_params {
+  int32_t dtype;          /* x, z, y, dy, dx, dz */
+  int32_t weight_dtype;   /* weight, bias, dweight, dbias: dtype or CC1D_F32 */
+  int32_t layer, gate_first;
+  int64_t rows, dim, group_size;
+  float eps;
+  int32_t _pad0;
+  const void* x;          int64_t x_row_stride;
+  const void* z;          int64_t z_row_stride;   /* NULL: no gate */
+  const void* weight;
+  const void* bias;       /* NULL: none */
+  void* y;                int64_t y_row_stride;   /* forward */
+  float* mean;            /* forward: NULL to skip; backward with layer: required */
+  float* rstd;
+  const void* dy;         int64_t dy_row_stride;  /* backward, from here on */
+  void* dx;               int64_t dx_row_stride;
+  void* dz;               int64_t dz_row_stride;  /* required iff z */
+  void* dweight;
+  void* dbias;            /* required iff bias */
+  void* workspace;        size_t workspace_bytes;
+} cc1d_gated_norm_params;
+
+CC1D_API int cc1d_gated_norm_fwd(const cc1d_gated_norm_params* params, void* stream);
+CC1D_API int cc1d_gated_norm_workspace_size(const cc1d_gated_norm_params* params, size_t* bytes);
+CC1D_API int cc1d_gated_norm_bwd(const cc1d_gated_norm_params* params, void* stream);
+
 /* Diagnostics: *wait_timeouts receives the number of bounded in-kernel waits
  * (pipeline barriers, peer exchanges) that gave up since the previous call,
  * and the count is reset.  The count is kept per device and this call reads
