@@ -423,6 +423,27 @@ int plan_scan(const cc1d_scan_params* p, ScanArgs* a, ScanPlan* plan) {
   a->seg_len = std::max<i64>(1, p->seqlen);
   a->segs = 1;
   a->items = nseq;
+  if (nseq == 0 || p->seqlen == 0) return CC1D_OK;
+  // The tensor cores work in blocks of 128 tokens: below 16 tokens a sequence
+  // the walk over tokens is done sooner.
+  const i64 mean = p->cu_seqlens ? ceil_div(p->seqlen, nseq) : p->seqlen;
+  plan->tc = mean >= 16 && scan_tc_eligible(p->dtype, *a, p->batch);
+  // Sequences are split when their rows alone do not fill the SMs (one CTA
+  // each on the tensor cores, about four blocks of the walk), into segments of
+  // two blocks or 64 tokens at least; packed ones as if they were one.
+  const i64 rows = (p->cu_seqlens ? 1 : nseq) * (plan->tc ? scan_tc_pairs(*a) : a->H * ceil_div(a->P, 64));
+  const i64 least = plan->tc ? 2 * kScanBlock : 64, unit = plan->tc ? kScanBlock : 16;
+  const i64 segs = std::min<i64>((plan->tc ? 148 : 592) / rows, p->seqlen / least);
+  if (segs > 1) {
+    const i64 len = ceil_div(ceil_div(p->seqlen, segs), unit) * unit;
+    const i64 longest = p->cu_seqlens && p->max_seqlen == 0 ? p->seqlen : p->cu_seqlens ? p->max_seqlen : p->seqlen;
+    if (longest > len) {
+      plan->split = true;
+      a->seg_len = len;
+      a->segs = (int)ceil_div(p->seqlen, len);
+      a->items = p->cu_seqlens ? nseq + p->seqlen / len : nseq * a->segs;
+    }
+  }
   return CC1D_OK;
 }
 
@@ -467,7 +488,9 @@ extern "C" int cc1d_scan(const cc1d_scan_params* p, void* stream) {
   }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e = cudaSuccess;
-  if (a.nseq > 0)
+  if (plan.tc)
+    e = launch_scan_tc(p->dtype, a, p->batch, s);
+  else if (a.nseq > 0)
     e = p->dtype == CC1D_F16    ? launch_walk<__half>(a, plan.split, s)
         : p->dtype == CC1D_BF16 ? launch_walk<__nv_bfloat16>(a, plan.split, s)
                                 : launch_walk<float>(a, plan.split, s);

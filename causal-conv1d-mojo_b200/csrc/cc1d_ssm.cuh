@@ -109,8 +109,12 @@ __device__ __forceinline__ float scan_step(const ScanArgs& a, i64 off, float bia
   return a.softplus ? softplus_f(v) : v;
 }
 
-// Tensor-core scan (cc1d_ssm_tc.cu): what it takes, and its launch.
-bool scan_tc_eligible(int dtype, const ScanArgs& a);
-cudaError_t launch_scan_tc(int dtype, const ScanArgs& a, cudaStream_t stream);
+// Tensor-core scan (cc1d_ssm_tc.cu): what it takes, the CTAs it runs per
+// segment, its tokens per block and its launch (the partial states first when
+// `part` is set).
+constexpr int kScanBlock = 128;
+bool scan_tc_eligible(int dtype, const ScanArgs& a, i64 batch);
+int scan_tc_pairs(const ScanArgs& a);
+cudaError_t launch_scan_tc(int dtype, const ScanArgs& a, i64 batch, cudaStream_t stream);
 
 }  // namespace cc1d
