@@ -102,10 +102,15 @@ __device__ __forceinline__ bool scan_locate(const ScanArgs& a, i64 item, ScanIte
 // log(1 + exp(v)), v itself where the two agree in fp32.
 __device__ __forceinline__ float softplus_f(float v) { return v > 20.f ? v : log1pf(expf(v)); }
 
-// The step length of a token: dt + bias, through softplus on request.
+// A token's dt as it is stored, and the step length: dt + bias, through
+// softplus on request.
+template <typename T>
+__device__ __forceinline__ float scan_raw_step(const ScanArgs& a, i64 off) {
+  return a.dt_f32 ? static_cast<const float*>(a.dt)[off] : Cvt<T>::f(static_cast<const T*>(a.dt)[off]);
+}
 template <typename T>
 __device__ __forceinline__ float scan_step(const ScanArgs& a, i64 off, float bias) {
-  const float v = (a.dt_f32 ? static_cast<const float*>(a.dt)[off] : Cvt<T>::f(static_cast<const T*>(a.dt)[off])) + bias;
+  const float v = scan_raw_step<T>(a, off) + bias;
   return a.softplus ? softplus_f(v) : v;
 }
 

@@ -38,25 +38,30 @@
 //
 // Roles (20 warps, one CTA per SM):
 //   warp 0       TMA: B and X in rings of two blocks, C in one buffer
-//                (released as soon as G and inter have read it)
-//   warp 1       allocates TMEM, issues every tcgen05.mma (one lane)
-//   warp 2       step lengths and decay factors of the next block
-//   warps 4-11   tokens: thread = token row.  M from G, in place in TMEM (a
-//                block of 32 fp32 columns becomes 16 + 16 columns, one head
-//                each); scales inter by exp(c_i), so that intra accumulates
-//                onto it; y + D x over x in shared memory, then out
+//                (released as soon as G and inter have read it); y out
+//   warp 1       allocates TMEM, issues G, inter and intra (one lane)
+//   warp 2       issues dS: the chains of y and of the state meet only where
+//                one needs the other, and one issuer for both would make each
+//                wait for the other's barriers
+//   warp 3       step lengths and decay factors of the next block
+//   warps 4-11   tokens: thread = token row.  M from G, in place in TMEM (16
+//                fp32 columns become 8 + 8 of pairs, one head each); scales inter by exp(c_i), so that intra accumulates
+//                onto it; y + D x over x in shared memory
 //   warps 12-19  state: thread = row p of S, half of n.  (w X)^T into TMEM,
 //                S = exp(c_Q) S + dS, 16-bit copy to shared memory
-// TMEM (512 columns): G / M 128, y 128, dS 128, (w X)^T 4 slots of 32 (64
-// tokens each).  (w X)^T comes from TMEM and not from shared memory because
+// TMEM (512 columns): G / M 128, y 128, dS 128, (w X)^T two buffers of one
+// unit (32 tokens, 16 columns a term).  (w X)^T comes from TMEM and not from shared memory because
 // the products' operands already take most of the shared-memory bandwidth.
-// Order of the products of block b: first half of dS, G, inter, rest of dS,
-// intra; so M is computed while dS runs, and the state is updated while
-// intra runs.
+// What a role does between two waits is kept short: with few warps it runs at
+// the latency of its instructions.
 //
-// Every mbarrier wait is bounded; a wait that gives up sets an abort flag
-// and ends its role, the others' waits then give up in turn, outstanding
-// copies and products are waited for (bounded) and TMEM is released.
+// A barrier tells only the last two phases apart, so one that its waiter
+// might see two blocks late is kept per stage.
+//
+// Every mbarrier wait is bounded; after one that gave up no wait waits, the
+// roles run to their ends, outstanding copies and products are waited for
+// (bounded), TMEM is released and the launch is counted in
+// cc1d_device_status.
 #include <cudaTypedefs.h>
 
 #include <algorithm>
@@ -102,9 +107,10 @@ struct Bars {
   uint64_t emptyB[2], emptyX[2], emptyC;
   uint64_t cumF[2], cumE[2];
   uint64_t gR, iR, pR, yR, yF;
-  uint64_t wR[4], wF[4];
-  uint64_t dR, dF, sR, end;
-  uint64_t ySync, xSync, mSync;  // among the token warps, among the state warps
+  uint64_t wR[2], wF[2];
+  uint64_t dR, dF, sR, end, endS;
+  uint64_t xF[2], yS[2];  // the state's warps have read x; y is in its place
+  uint64_t xSync, mSync;  // among the state warps
   uint32_t tmem;
   int abort;
 };
@@ -115,7 +121,7 @@ static_assert(kOffCum % 16 == 0 && sizeof(Cum) % 16 == 0 && kOffBar % 8 == 0, "a
 constexpr uint32_t kColG = 0, kColY = 128, kColD = 256, kColW = 384;
 
 struct alignas(64) TcArgs {
-  CUtensorMap mx, mb, mc;
+  CUtensorMap mx, mb, mc, my;
   ScanArgs a;
   int npairs, ppg;   // CTAs per segment; per group
   int nb;            // 64-column blocks of the state size
@@ -149,25 +155,20 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc)
       : "memory");
 }
-__device__ __forceinline__ void tm_ld32(uint32_t t, uint32_t (&r)[32]) {
+__device__ __forceinline__ void tm_ld16(uint32_t t, uint32_t (&r)[16]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+      "[%16];"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(t)
       : "memory");
 }
-__device__ __forceinline__ void tm_st32(uint32_t t, const uint32_t (&r)[32]) {
+__device__ __forceinline__ void tm_st16(uint32_t t, const uint32_t (&r)[16]) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::"r"(r[0]), "r"(r[1]),
-      "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
-      "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]),
-      "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]),
-      "r"(r[30]), "r"(r[31]), "r"(t)
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(t)
       : "memory");
 }
 __device__ __forceinline__ void tm_st8(uint32_t t, const uint32_t (&r)[8]) {
@@ -175,6 +176,11 @@ __device__ __forceinline__ void tm_st8(uint32_t t, const uint32_t (&r)[8]) {
       "tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]),
       "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(t)
       : "memory");
+}
+__device__ __forceinline__ void tm_st4(uint32_t t, const uint32_t (&r)[4]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%4], {%0, %1, %2, %3};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]),
+               "r"(r[3]), "r"(t)
+               : "memory");
 }
 __device__ __forceinline__ void tm_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tm_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -202,21 +208,58 @@ __device__ __forceinline__ void tma_tile(void* dst, const CUtensorMap* map, uint
       : "memory");
 }
 
-// Bounded wait that also gives up when another role has.
-__device__ __forceinline__ bool wait_or_abort(uint64_t* bar, unsigned parity, volatile int* abort_flag) {
-  for (unsigned i = 0; i < kSpinLimit; ++i) {
-    if (mbar_try_wait(bar, parity)) return true;
-    if ((i & 255u) == 255u && *abort_flag) return false;
-  }
-  atomicAdd(&g_cc1d_wait_timeouts, 1u);
-  *abort_flag = 1;
-  return false;
+// Bounded wait by a warp (or one lane).  One that gives up sets the abort
+// flag, and with the flag set no wait waits: every role then runs to its end
+// on whatever is there, within its buffers, and the kernel is over.
+__device__ __forceinline__ void wait_for(uint64_t* bar, unsigned parity, int* abort_flag) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .u32 n, f;\n\t"
+      "mov.u32 n, %2;\n\t"
+      "W%=: mbarrier.try_wait.parity.shared::cta.b64 p, [%0], %1;\n\t"
+      "@p bra D%=;\n\t"
+      "ld.volatile.shared.u32 f, [%3];\n\t"
+      "setp.ne.u32 p, f, 0;\n\t@p bra D%=;\n\t"
+      "sub.u32 n, n, 1;\n\tsetp.ne.u32 p, n, 0;\n\t@p bra W%=;\n\t"
+      "st.volatile.shared.u32 [%3], 1;\n\t"
+      "D%=:\n\t}" ::"r"(smem_u32(bar)),
+      "r"(parity), "n"(kSpinLimit), "r"(smem_u32(abort_flag))
+      : "memory");
+}
+
+__device__ __forceinline__ void tma_store(const CUtensorMap* map, const void* src, int c0, int c1, int c2, int c3) {
+  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(smem_u32(src)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+               : "memory");
 }
 
 // One vote of a warp: all its lanes' accesses before are ordered before it.
 __device__ __forceinline__ void warp_arrive(uint64_t* bar) {
   __syncwarp();
-  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.eq.u32 p, %1, 0;\n\t"
+      "@p mbarrier.arrive.shared::cta.b64 _, [%0];\n\t}" ::"r"(smem_u32(bar)),
+      "r"(threadIdx.x & 31)
+      : "memory");
+}
+
+// Takes the leading 16-bit term off two values.  bf16 terms of a split are
+// cut, not rounded: the upper halves of the words, eight bits each, so that
+// three of them are the 24 bits of the value.
+template <typename T, bool SPLIT>
+__device__ __forceinline__ uint32_t take_term(float2& v) {
+  if constexpr (!SPLIT) {
+    return Pair<T>::pack(v);
+  } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    const uint32_t a = __float_as_uint(v.x), b = __float_as_uint(v.y);
+    v = add2(v, f2(__uint_as_float((a & 0xffff0000u) ^ 0x80000000u), __uint_as_float((b & 0xffff0000u) ^ 0x80000000u)));
+    return __byte_perm(a, b, 0x7632);
+  } else {
+    const uint32_t w = Pair<T>::pack(v);
+    const float2 back = Pair<T>::unpack(w);
+    v = add2(v, f2(-back.x, -back.y));
+    return w;
+  }
 }
 
 // TERMS: 16-bit terms of w X.  PART: only the segment's state from zero.
@@ -224,10 +267,10 @@ __device__ __forceinline__ void warp_arrive(uint64_t* bar) {
 template <typename T, int TERMS, bool PART, bool WIDE>
 __global__ void __launch_bounds__(kThreads, 1) scan_tc_kernel(const __grid_constant__ TcArgs p) {
   extern __shared__ unsigned char smem_raw[];
-  unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  // An offset, not a rounded pointer, so that accesses stay shared-memory ones.
+  unsigned char* sm = smem_raw + (-smem_u32(smem_raw) & 1023u);
   Bars* bar = reinterpret_cast<Bars*>(sm + kOffBar);
   Cum(*cum)[2] = reinterpret_cast<Cum(*)[2]>(sm + kOffCum);  // [stage][head]
-  volatile int* abort_flag = &bar->abort;
   const ScanArgs& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -246,9 +289,11 @@ __global__ void __launch_bounds__(kThreads, 1) scan_tc_kernel(const __grid_const
     for (int s = 0; s < 2; ++s) {
       mbar_init(&bar->fullB[s], 1);
       mbar_init(&bar->fullX[s], 1);
-      mbar_init(&bar->emptyB[s], 1);
+      mbar_init(&bar->emptyB[s], PART ? 1 : 2);  // both issuers
       mbar_init(&bar->emptyX[s], 8);
       mbar_init(&bar->cumF[s], 1);
+      mbar_init(&bar->xF[s], 8);
+      mbar_init(&bar->yS[s], 8);
       mbar_init(&bar->cumE[s], PART ? 8 : 16);
     }
     mbar_init(&bar->fullC, 1);
@@ -258,7 +303,7 @@ __global__ void __launch_bounds__(kThreads, 1) scan_tc_kernel(const __grid_const
     mbar_init(&bar->pR, 8);
     mbar_init(&bar->yR, 1);
     mbar_init(&bar->yF, 8);
-    for (int s = 0; s < 4; ++s) {
+    for (int s = 0; s < 2; ++s) {
       mbar_init(&bar->wR[s], 8);
       mbar_init(&bar->wF[s], 1);
     }
@@ -266,7 +311,7 @@ __global__ void __launch_bounds__(kThreads, 1) scan_tc_kernel(const __grid_const
     mbar_init(&bar->dF, 8);
     mbar_init(&bar->sR, 8);
     mbar_init(&bar->end, 1);
-    mbar_init(&bar->ySync, 8);
+    mbar_init(&bar->endS, 1);
     mbar_init(&bar->xSync, 8);
     mbar_init(&bar->mSync, 8);
     bar->abort = 0;
@@ -277,168 +322,252 @@ __global__ void __launch_bounds__(kThreads, 1) scan_tc_kernel(const __grid_const
   __syncthreads();
   tc_after();
   const uint32_t tmem = bar->tmem;
-  // A wait that gave up ends its role (for a whole warp: of all its lanes).
-#define CC1D_WAIT1(b, ph)                                  \
-  if (!wait_or_abort(&bar->b, (ph)&1, abort_flag)) break;
-#define CC1D_WAITW(b, ph)                                                      \
-  if (__any_sync(kFull, !wait_or_abort(&bar->b, (ph)&1, abort_flag))) break;
+  auto wait = [&](uint64_t& b, unsigned phase) { wait_for(&b, phase & 1, &bar->abort); };
 
+  // Registers: 96 a thread at launch (61440 in all); the state's warps take
+  // over what the first four do not need (4 * 32 * 64 + 8 * 32 * 96 +
+  // 8 * 32 * 112 = 61440).
+  if (warp < 4) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
   if (warp == 0) {
     // ---------------- TMA ----------------
     if (lane == 0) {
       prefetch_tensormap(&p.mx);
       prefetch_tensormap(&p.mb);
-      if (!PART) prefetch_tensormap(&p.mc);
-      unsigned nB = 0, nX = 0, nC = 0;  // loads issued
-      for (unsigned c = 0; c < (unsigned)nblk; ++c) {
+      if (!PART) {
+        prefetch_tensormap(&p.mc);
+        prefetch_tensormap(&p.my);
+      }
+      const int b = (int)it.batch;
+      const int np = WIDE ? 2 : nh;  // boxes of y
+      // y of block c, out of x's buffer, which is free afterwards.  A block
+      // that its sequence fills in part is stored by the tokens' warps.
+      auto store = [&](unsigned c) {
         const unsigned s = c & 1;
-        const int t = (int)(it.t0 + (i64)c * kQ), b = (int)it.batch;
-        if (c >= 2) { CC1D_WAIT1(emptyB[s], (c >> 1) - 1) }
+        const i64 t = it.t0 + (i64)c * kQ;
+        wait(bar->yS[s], c >> 1);
+        if (a.cu != nullptr && it.t1 - t < kQ) return;
+#pragma unroll 1
+        for (int k = 0; k < np; ++k)
+          tma_store(&p.my, sm + kOffX + s * kTile + k * kBox, WIDE ? 64 * k : 0, WIDE ? h0 : h0 + k, (int)t, b);
+        asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group.read 0;" ::: "memory");
+      };
+      int t = (int)it.t0;
+#pragma unroll 1
+      for (unsigned c = 0; c < (unsigned)nblk; ++c, t += kQ) {
+        const unsigned s = c & 1;
+        if (c >= 2) wait(bar->emptyB[s], (c >> 1) - 1);
         mbar_arrive_expect_tx(&bar->fullB[s], p.nb * kBox);
+#pragma unroll 1
         for (int k = 0; k < p.nb; ++k) tma_tile(sm + kOffB + s * kTile + k * kBox, &p.mb, &bar->fullB[s], 64 * k, g, t, b);
-        ++nB;
-        if (!PART) {
-          if (c >= 1) { CC1D_WAIT1(emptyC, c - 1) }
-          mbar_arrive_expect_tx(&bar->fullC, p.nb * kBox);
-          for (int k = 0; k < p.nb; ++k) tma_tile(sm + kOffC + k * kBox, &p.mc, &bar->fullC, 64 * k, g, t, b);
-          ++nC;
+        if (c >= 2) {
+          if (PART)
+            wait(bar->emptyX[s], (c >> 1) - 1);
+          else
+            store(c - 2);
         }
-        if (c >= 2) { CC1D_WAIT1(emptyX[s], (c >> 1) - 1) }
         mbar_arrive_expect_tx(&bar->fullX[s], kTile);
+#pragma unroll 1
         for (int k = 0; k < 2; ++k)
           tma_tile(sm + kOffX + s * kTile + k * kBox, &p.mx, &bar->fullX[s], WIDE ? 64 * k : 0, WIDE ? h0 : h0 + k, t, b);
-        ++nX;
+        if (!PART) {
+          if (c >= 1) wait(bar->emptyC, c - 1);
+          mbar_arrive_expect_tx(&bar->fullC, p.nb * kBox);
+#pragma unroll 1
+          for (int k = 0; k < p.nb; ++k) tma_tile(sm + kOffC + k * kBox, &p.mc, &bar->fullC, 64 * k, g, t, b);
+        }
       }
-      // Nothing may land after the block has gone (normally all has landed).
-      mbar_drain(bar->fullB, nB, 2);
-      mbar_drain(bar->fullX, nX, 2);
-      if (!PART) mbar_drain(&bar->fullC, nC, 1);
+      if (!PART) {
+        if (nblk > 1) store(nblk - 2);
+        if (nblk > 0) store(nblk - 1);
+      }
+      // Nothing may land after the CTA has gone (normally all has landed).
+      mbar_drain(bar->fullB, nblk, 2);
+      mbar_drain(bar->fullX, nblk, 2);
+      if (!PART) mbar_drain(&bar->fullC, nblk, 1);
     }
   } else if (warp == 1) {
-    // ---------------- matrix products ----------------
-    if (lane == 0) {
-      const uint32_t sB = smem_u32(sm + kOffB), sX = smem_u32(sm + kOffX), sC = smem_u32(sm + kOffC), sS = smem_u32(sm + kOffS);
-      const uint32_t dG = tmem + kColG, dY = tmem + kColY, dD = tmem + kColD, dW = tmem + kColW;
+    // ---------------- products of y: G, inter, intra ----------------
+    // A whole warp walks the loop, so that descriptors are uniform; one lane
+    // issues.
+    if (!PART) {
+      const bool lead = lane == 0;
+      const uint32_t sm0 = smem_u32(sm);
+      const uint32_t dG = tmem + kColG, dY = tmem + kColY;
       const uint32_t id_nn = i_desc<T>(128, false);             // G, inter
       const uint32_t id_in = i_desc<T>(WIDE ? 128 : 64, true);  // intra
-      const uint32_t id_st = i_desc<T>(64 * p.nb, true);        // dS
-      const int ksteps = 4 * p.nb;
-      unsigned n = 0;  // slots of w X used
+      const uint64_t kC = sw_desc(sm0 + kOffC, 16), kB = sw_desc(sm0 + kOffB, 16), kS = sw_desc(sm0 + kOffS, 16);
+      const uint64_t mX = sw_desc(sm0 + kOffX, kBox);
+      // D = C (K-major rows of Q) with a K-major B operand, K = the state size.
+      auto by_state = [&](uint32_t d, uint64_t b) {
+        uint64_t ca = kC;
+#pragma unroll 1
+        for (int k = 0; k < 2 * p.nb; ++k) {
+          if (lead) {
+            mma_ss(d, ca, b, id_nn, k != 0);
+            mma_ss(d, ca + 2, b + 2, id_nn, 1);
+          }
+          // 32 bytes a step; the next 64 columns are in the next box.
+          const uint32_t o = k == 1 ? (kBox - 64) >> 4 : 4;
+          ca += o;
+          b += o;
+        }
+      };
+#pragma unroll 1
       for (unsigned c = 0; c < (unsigned)nblk; ++c) {
         const unsigned s = c & 1;
-        bool ok = true;
-        // dS += (term, 64 tokens) of each slot; two halves of TERMS slots.
-        auto state = [&](int from, int to) {
-          for (int k = from; k < to && ok; ++k, ++n) {
-            const unsigned sl = n & 3;
-            ok = wait_or_abort(&bar->wR[sl], (n >> 2) & 1, abort_flag);
-            if (!ok) return;
-            tc_after();
-            const int half = k / TERMS;
-#pragma unroll
-            for (int ks = 0; ks < 4; ++ks)
-              mma_ts(dD, dW + sl * 32 + ks * 8, sw_desc(sB + s * kTile + (half * 4 + ks) * 2048, kBox), id_st, (k | ks) != 0);
-            tc_commit(&bar->wF[sl]);
-          }
-        };
-        CC1D_WAIT1(fullB[s], c >> 1)
-        if (c > 0) { CC1D_WAIT1(dF, c - 1) }
+        wait(bar->fullB[s], c >> 1);
+        wait(bar->fullC, c);
+        if (c > 0) wait(bar->yR, c - 1);  // intra of the block before reads M where G goes
         tc_after();
-        if (TERMS > 1 || PART) state(0, TERMS);
-        if (!ok) break;
-        if (!PART) {
-          CC1D_WAIT1(fullC, c)
-          // intra of the block before reads M where G goes.
-          if (c > 0) { CC1D_WAIT1(yR, c - 1) }
-          tc_after();
-          for (int ks = 0; ks < ksteps; ++ks) {
-            const uint32_t o = (ks >> 2) * kBox + (ks & 3) * 32;
-            mma_ss(dG, sw_desc(sC + o, 16), sw_desc(sB + s * kTile + o, 16), id_nn, ks != 0);
-          }
+        by_state(dG, kB + ((s * kTile) >> 4));
+        if (lead) {
           tc_commit(&bar->gR);
-          CC1D_WAIT1(sR, c)
-          if (c > 0) { CC1D_WAIT1(yF, c - 1) }
-          tc_after();
-          for (int ks = 0; ks < ksteps; ++ks) {
-            const uint32_t o = (ks >> 2) * kBox + (ks & 3) * 32;
-            mma_ss(dY, sw_desc(sC + o, 16), sw_desc(sS + o, 16), id_nn, ks != 0);
-          }
+          tc_commit(&bar->emptyB[s]);
+        }
+        wait(bar->sR, c);
+        if (c > 0) wait(bar->yF, c - 1);
+        tc_after();
+        by_state(dY, kS);
+        if (lead) {
           tc_commit(&bar->iR);
           tc_commit(&bar->emptyC);
         }
-        state(TERMS > 1 || PART ? TERMS : 0, 2 * TERMS);
-        if (!ok) break;
-        tc_commit(&bar->dR);
-        tc_commit(&bar->emptyB[s]);
-        if (!PART) {
-          CC1D_WAIT1(pR, c)
-          CC1D_WAIT1(fullX[s], c >> 1)
-          tc_after();
-          for (int hs = 0; hs < (WIDE ? 1 : 2); ++hs)
-            for (int ks = 0; ks < 8; ++ks)
-              mma_ts(dY + hs * 64, dG + 32 * (ks >> 1) + 16 * hs + 8 * (ks & 1),
-                     sw_desc(sX + s * kTile + hs * kBox + ks * 2048, kBox), id_in, 1);
-          tc_commit(&bar->yR);
+        wait(bar->fullX[s], c >> 1);
+        if (a.cu != nullptr && it.t1 - it.t0 - (i64)c * kQ < kQ) wait(bar->xSync, 0);  // foreign rows are zeros
+        wait(bar->pR, c);
+        tc_after();
+        // Head slot k >> 2, tokens [32 (k & 3), + 32).
+        uint64_t b = mX + ((s * kTile) >> 4);
+#pragma unroll 1
+        for (int k = 0; k < (WIDE ? 4 : 8); ++k, b += 4096u >> 4) {
+          if (lead) {
+            const uint32_t m = dG + 32 * (k & 3) + 8 * (k >> 2);
+            mma_ts(dY + 64 * (k >> 2), m, b, id_in, 1);
+            mma_ts(dY + 64 * (k >> 2), m + 16, b + (2048u >> 4), id_in, 1);
+          }
         }
+        if (lead) tc_commit(&bar->yR);
       }
-      if (nblk > 0) {  // the block stays until its last products are done
-        tc_commit(&bar->end);
-        (void)mbar_wait(&bar->end, 0);
+      if (nblk > 0) {  // the CTA stays until its last products are done
+        if (lead) tc_commit(&bar->end);
+        wait(bar->end, 0);
       }
     }
   } else if (warp == 2) {
-    // ---------------- steps and decays ----------------
-    float A2[2], bias[2];
-    for (int k = 0; k < 2; ++k) {
-      const bool ok = k < nh;
-      A2[k] = ok ? a.A[h0 + k] * kLog2e : 0.f;
-      bias[k] = ok && a.dt_bias ? a.dt_bias[h0 + k] : 0.f;
-    }
-    const i64 o = it.batch * a.ds_b + h0 * a.ds_h;
+    // ---------------- products of the state: dS ----------------
+    const bool lead = lane == 0;
+    const uint32_t dD = tmem + kColD, dW = tmem + kColW;
+    const uint32_t id_st = i_desc<T>(64 * p.nb, true);
+    const uint64_t mB = sw_desc(smem_u32(sm) + kOffB, kBox);
+#pragma unroll 1
     for (unsigned c = 0; c < (unsigned)nblk; ++c) {
       const unsigned s = c & 1;
-      float d[2][4];
+      wait(bar->fullB[s], c >> 1);
+      if (c > 0) wait(bar->dF, c - 1);
+      // Units of 32 tokens, TERMS terms each.
+#pragma unroll 1
+      for (unsigned u = 0; u < 4; ++u) {
+        const unsigned n = 4 * c + u;
+        wait(bar->wR[n & 1], n >> 1);
+        tc_after();
+        const uint64_t b = mB + ((s * kTile + u * 4096u) >> 4);
+        uint32_t w = dW + (n & 1) * (16 * TERMS);
+#pragma unroll 1
+        for (int k = 0; k < TERMS; ++k, w += 16) {
+          if (lead) {
+            mma_ts(dD, w, b, id_st, (k | u) != 0);
+            mma_ts(dD, w + 8, b + (2048u >> 4), id_st, 1);
+          }
+        }
+        if (lead) tc_commit(&bar->wF[n & 1]);
+      }
+      if (lead) {
+        tc_commit(&bar->dR);
+        tc_commit(&bar->emptyB[s]);
+      }
+    }
+    if (nblk > 0) {
+      if (lead) tc_commit(&bar->endS);
+      wait(bar->endS, 0);
+    }
+  } else {
+    // ---------------- steps and decays ----------------
+    const i64 o = it.batch * a.ds_b + h0 * a.ds_h;
+    constexpr int kH = WIDE ? 1 : 2;
+    const int es = a.dt_f32 ? 4 : (int)sizeof(T);
+    const char* dp = static_cast<const char*>(a.dt) + (o + (it.t0 + lane) * a.ds_t) * es;
+    const i64 hstep = a.ds_h * es, tstep = 32 * a.ds_t * es;
+    // dt of the lane's four tokens, both heads; the next block's are on their
+    // way while this one's are worked on.
+    auto load = [&](unsigned c, float (&d)[kH][4]) {
+      const i64 left = it.t1 - it.t0 - (i64)c * kQ - lane;
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
+      for (int k = 0; k < kH; ++k) {
+        const char* q4 = dp + k * hstep;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const i64 t = it.t0 + (i64)c * kQ + q * 32 + lane;
-          d[k][q] = k < nh && t < it.t1 ? scan_step<T>(a, o + k * a.ds_h + t * a.ds_t, bias[k]) : 0.f;
+        for (int q = 0; q < 4; ++q, q4 += tstep) {
+          d[k][q] = 0.f;
+          if (k < nh && left > 32 * q)
+            d[k][q] = a.dt_f32 ? *reinterpret_cast<const float*>(q4) : Cvt<T>::f(*reinterpret_cast<const T*>(q4));
         }
       }
-      if (c >= 2) { CC1D_WAITW(cumE[s], (c >> 1) - 1) }
-      for (int k = 0; k < (WIDE ? 1 : 2); ++k) {
+      dp += 4 * tstep;
+    };
+    float d[kH][4];
+    if (nblk > 0) load(0, d);
+#pragma unroll 1
+    for (unsigned c = 0; c < (unsigned)nblk; ++c) {
+      const unsigned s = c & 1;
+      if (c >= 2) wait(bar->cumE[s], (c >> 1) - 1);
+#pragma unroll
+      for (int k = 0; k < kH; ++k) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) cum[s][k].d[q * 32 + lane] = d[k][q];
+      }
+      if (c + 1 < (unsigned)nblk) load(c + 1, d);
+      const int left = (int)min(it.t1 - it.t0 - (i64)c * kQ, (i64)kQ) - lane;
+#pragma unroll 1
+      for (int k = 0; k < kH; ++k) {
         Cum& u = cum[s][k];
+        const bool head = k < nh;
+        const float A2 = head ? a.A[h0 + k] * kLog2e : 0.f, bias = head && a.dt_bias ? a.dt_bias[h0 + k] : 0.f;
         float l[4], r[4], tot[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const float v = fmaxf(d[k][q] * A2[k], -160.f);
-          l[q] = v;
-          r[q] = v;
+          // Tokens behind the end, and a head that is not there: steps of length 0.
+          float d1 = u.d[q * 32 + lane] + bias;
+          d1 = !head || left <= 32 * q ? 0.f : a.softplus ? softplus_f(d1) : d1;
+          u.d[q * 32 + lane] = d1;
+          l[q] = r[q] = fmaxf(d1 * A2, -160.f);
+        }
 #pragma unroll
-          for (int sh = 1; sh < 32; sh <<= 1) {
+        for (int sh = 1; sh < 32; sh <<= 1) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
             const float up = __shfl_up_sync(kFull, l[q], sh), dn = __shfl_down_sync(kFull, r[q], sh);
             if (lane >= sh) l[q] += up;
             if (lane + sh < 32) r[q] += dn;
           }
+        }
+        float before[4], after[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
           tot[q] = __shfl_sync(kFull, r[q], 0);
           r[q] = __shfl_down_sync(kFull, r[q], 1);
           if (lane == 31) r[q] = 0.f;
         }
+        before[0] = 0.f, before[1] = tot[0], before[2] = tot[0] + tot[1], before[3] = before[2] + tot[2];
+        after[3] = 0.f, after[2] = tot[3], after[1] = tot[2] + tot[3], after[0] = tot[1] + after[1];
         float w[4], big = 0.f;
-        float before = 0.f;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          float later = 0.f;
-#pragma unroll
-          for (int j = 3; j > q; --j) later += tot[j];
           const int t = q * 32 + lane;
+          const float d1 = u.d[t];
           u.l[t] = l[q];
-          u.d[t] = d[k][q];
-          u.u[t] = d[k][q] * ex2_approx(r[q]);
-          w[q] = d[k][q] * ex2_approx(r[q] + later);
-          u.e[t] = ex2_approx(before + l[q]);
-          before += tot[q];
+          u.u[t] = d1 * ex2_approx(r[q]);
+          w[q] = d1 * ex2_approx(r[q] + after[q]);
+          u.e[t] = ex2_approx(before[q] + l[q]);
           big = fmaxf(big, fabsf(w[q]));
         }
         // fp16, one term: the largest weight into [1/2, 1), so that w x cannot overflow.
@@ -452,16 +581,16 @@ __global__ void __launch_bounds__(kThreads, 1) scan_tc_kernel(const __grid_const
         }
 #pragma unroll
         for (int q = 0; q < 4; ++q) u.w[q * 32 + lane] = w[q] * scale;
+        if (lane < 4) u.tot[lane] = lane == 0 ? tot[0] : lane == 1 ? tot[1] : lane == 2 ? tot[2] : tot[3];
         if (lane == 0) {
-#pragma unroll
-          for (int q = 0; q < 4; ++q) u.tot[q] = tot[q];
-          u.dec = ex2_approx(before);
+          u.dec = ex2_approx(before[3] + tot[3]);
           u.unscale = unscale;
         }
       }
       warp_arrive(&bar->cumF[s]);
     }
-  } else if (warp >= 4 && warp < 12) {
+  }
+  } else if (warp < 12) {
     // ---------------- tokens ----------------
     if (!PART) {
       const int q = warp & 3, hf = (warp - 4) >> 2;
@@ -470,136 +599,132 @@ __global__ void __launch_bounds__(kThreads, 1) scan_tc_kernel(const __grid_const
       const int hs = WIDE ? 0 : hf;  // head slot of this thread's y columns
       const int yt = threadIdx.x - 128;
       const float Dh = a.D && hs < nh ? a.D[h0 + hs] : 0.f;
+#pragma unroll 1
       for (unsigned c = 0; c < (unsigned)nblk; ++c) {
         const unsigned s = c & 1;
-        CC1D_WAITW(cumF[s], c >> 1)
+        wait(bar->cumF[s], c >> 1);
         const Cum* cu = cum[s];
-        CC1D_WAITW(gR, c)
+        // M: this thread's row, 16 columns of each sub-block; the two warps
+        // of a row share every sub-block, so the causal work is even.  16
+        // fp32 columns become 8 + 8 columns of 16-bit pairs, one head each.
+        constexpr int kH = WIDE ? 1 : 2;
+        const uint32_t atG = tmem + lanes + kColG + 16 * hf;
+        wait(bar->gR, c);
         tc_after();
-        // M: this thread's row, sub-blocks {0, 3} or {1, 2} of the columns
-        // (which shares the causal work evenly).
+        uint32_t v[16];
+        tm_ld16(atG + 32 * q, v);
+        tm_ld_wait();
+        const int last = lane - 16 * hf;  // last unmasked column of the row's own sub-block
 #pragma unroll 1
-        for (int bi = 0; bi < 2; ++bi) {
-          const int b = hf == 0 ? bi * 3 : 1 + bi;
-          uint32_t v[32];
-          const uint32_t at = tmem + lanes + kColG + 32 * b;
-          if (b > q) {
+        for (int k = 0; k < kH; ++k) {
+          const Cum& u = cu[k];
+          const float l = u.l[row];
+          const float4* lp = reinterpret_cast<const float4*>(u.l + 32 * q + 16 * hf);
+          const float4* dp = reinterpret_cast<const float4*>(u.d + 32 * q + 16 * hf);
+          uint32_t o[8];
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = 0u;
-          } else {
-            tm_ld32(at, v);
-            tm_ld_wait();
-            uint32_t o[32];
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              if (WIDE && k == 1) {
-#pragma unroll
-                for (int j = 16; j < 32; ++j) o[j] = 0u;
-                break;
-              }
-              const Cum& u = cu[k];
-              if (b < q) {
-                float f = u.l[row];
-                for (int m = b + 1; m < q; ++m) f += u.tot[m];
-                f = ex2_approx(f);
-                const float2 ff = f2(f, f);
-                const float4* up = reinterpret_cast<const float4*>(u.u + 32 * b);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                  const float4 w4 = up[j];
-                  const float2 m0 = mul2(mul2(f2(__uint_as_float(v[4 * j]), __uint_as_float(v[4 * j + 1])), f2(w4.x, w4.y)), ff);
-                  const float2 m1 = mul2(mul2(f2(__uint_as_float(v[4 * j + 2]), __uint_as_float(v[4 * j + 3])), f2(w4.z, w4.w)), ff);
-                  o[16 * k + 2 * j] = Pair<T>::pack(m0);
-                  o[16 * k + 2 * j + 1] = Pair<T>::pack(m1);
-                }
-              } else {
-                const float li = u.l[row];
-                const float4* lp = reinterpret_cast<const float4*>(u.l + 32 * b);
-                const float4* dp = reinterpret_cast<const float4*>(u.d + 32 * b);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                  const float4 l4 = lp[j], d4 = dp[j];
-                  float m[4];
-                  const float lj[4] = {l4.x, l4.y, l4.z, l4.w}, dj[4] = {d4.x, d4.y, d4.z, d4.w};
-#pragma unroll
-                  for (int e = 0; e < 4; ++e)
-                    m[e] = 4 * j + e <= lane ? __uint_as_float(v[4 * j + e]) * (ex2_approx(li - lj[e]) * dj[e]) : 0.f;
-                  o[16 * k + 2 * j] = Pair<T>::pack(f2(m[0], m[1]));
-                  o[16 * k + 2 * j + 1] = Pair<T>::pack(f2(m[2], m[3]));
-                }
-              }
-            }
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = o[j];
+          for (int j = 0; j < 4; ++j) {
+            const float4 l4 = lp[j], d4 = dp[j];
+            const float m0 = 4 * j + 0 <= last ? __uint_as_float(v[4 * j + 0]) * (ex2_approx(l - l4.x) * d4.x) : 0.f;
+            const float m1 = 4 * j + 1 <= last ? __uint_as_float(v[4 * j + 1]) * (ex2_approx(l - l4.y) * d4.y) : 0.f;
+            const float m2 = 4 * j + 2 <= last ? __uint_as_float(v[4 * j + 2]) * (ex2_approx(l - l4.z) * d4.z) : 0.f;
+            const float m3 = 4 * j + 3 <= last ? __uint_as_float(v[4 * j + 3]) * (ex2_approx(l - l4.w) * d4.w) : 0.f;
+            o[2 * j] = Pair<T>::pack(f2(m0, m1));
+            o[2 * j + 1] = Pair<T>::pack(f2(m2, m3));
           }
-          tm_st32(at, v);
+          tm_st8(atG + 32 * q + 8 * k, o);
         }
+#pragma unroll 1
+        for (int b = q - 1; b >= 0; --b) {
+          tm_ld16(atG + 32 * b, v);
+          tm_ld_wait();
+#pragma unroll 1
+          for (int k = 0; k < kH; ++k) {
+            const Cum& u = cu[k];
+            // Decay from the end of sub-block b to the row.
+            float f = u.l[row];
+            for (int m = b + 1; m < q; ++m) f += u.tot[m];
+            f = ex2_approx(f);
+            const float2 ff = f2(f, f);
+            const float4* up = reinterpret_cast<const float4*>(u.u + 32 * b + 16 * hf);
+            uint32_t o[8];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float4 w4 = up[j];
+              o[2 * j] = Pair<T>::pack(mul2(mul2(f2(__uint_as_float(v[4 * j]), __uint_as_float(v[4 * j + 1])), f2(w4.x, w4.y)), ff));
+              o[2 * j + 1] = Pair<T>::pack(mul2(mul2(f2(__uint_as_float(v[4 * j + 2]), __uint_as_float(v[4 * j + 3])), f2(w4.z, w4.w)), ff));
+            }
+            tm_st8(atG + 32 * b + 8 * k, o);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) v[j] = 0u;
+#pragma unroll 1
+        for (int b = q + 1; b < 4; ++b) tm_st16(atG + 32 * b, v);
         // inter times exp(c_i), in place.
-        CC1D_WAITW(iR, c)
+        wait(bar->iR, c);
         tc_after();
         {
           const float e = cu[hs].e[row];
 #pragma unroll 1
-          for (int k = 0; k < 2; ++k) {
-            uint32_t v[32];
-            const uint32_t at = tmem + lanes + kColY + 64 * hf + 32 * k;
-            tm_ld32(at, v);
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t at = tmem + lanes + kColY + 64 * hf + 16 * k;
+            tm_ld16(at, v);
             tm_ld_wait();
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * e);
-            tm_st32(at, v);
+            for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * e);
+            tm_st16(at, v);
           }
         }
         tm_st_wait();
         tc_before();
         warp_arrive(&bar->pR);
-        if (lane == 0) mbar_arrive(&bar->cumE[s]);
+        warp_arrive(&bar->cumE[s]);
         // y + D x, over x.
-        CC1D_WAITW(yR, c)
+        wait(bar->yR, c);
+        wait(bar->xF[s], c >> 1);
         tc_after();
         uint4* xr = reinterpret_cast<uint4*>(sm + kOffX + s * kTile + hf * kBox + row * 128);
         const int sw = row & 7;
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          uint32_t v[32];
-          tm_ld32(tmem + lanes + kColY + 64 * hf + 32 * k, v);
+#pragma unroll 1
+        for (int k = 0; k < 4; ++k) {
+          tm_ld16(tmem + lanes + kColY + 64 * hf + 16 * k, v);
           tm_ld_wait();
-          if (k == 1) {
-            tc_before();
-            warp_arrive(&bar->yF);
-          }
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            uint4 w = xr[(4 * k + j) ^ sw];
+          for (int j = 0; j < 2; ++j) {
+            uint4 w = xr[(2 * k + j) ^ sw];
             uint32_t* wp = &w.x;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const float2 xv = Pair<T>::unpack(wp[e]);
-              wp[e] = Pair<T>::pack(f2(fmaf(Dh, xv.x, __uint_as_float(v[8 * j + 2 * e])),
-                                       fmaf(Dh, xv.y, __uint_as_float(v[8 * j + 2 * e + 1]))));
+              wp[e] = Pair<T>::pack(fma2(f2(Dh, Dh), xv, f2(__uint_as_float(v[8 * j + 2 * e]), __uint_as_float(v[8 * j + 2 * e + 1]))));
             }
-            xr[(4 * k + j) ^ sw] = w;
+            xr[(2 * k + j) ^ sw] = w;
           }
         }
-        warp_arrive(&bar->ySync);
-        CC1D_WAITW(ySync, c)
-        const i64 tb = it.t0 + (i64)c * kQ;
-        const int nv = (int)min((i64)kQ, it.t1 - tb);
-        T* y = static_cast<T*>(a.y) + it.batch * a.ys_b + tb * a.ys_t + h0 * a.ys_h;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const int e = yt + 256 * k, box = e >> 10, r = (e >> 3) & 127, un = e & 7;
-          const int col = (WIDE ? 64 * box : 0) + 8 * un;
-          if (r < nv && col < a.P && (WIDE || box < nh)) {
-            const uint4 w = *reinterpret_cast<const uint4*>(sm + kOffX + s * kTile + box * kBox + r * 128 + ((un ^ (r & 7)) << 4));
-            *reinterpret_cast<uint4*>(y + r * a.ys_t + (WIDE ? 0 : box * a.ys_h) + col) = w;
-          }
-        }
+        tc_before();
         fence_proxy_async_smem();
-        warp_arrive(&bar->emptyX[s]);
+        warp_arrive(&bar->yF);
+        warp_arrive(&bar->yS[s]);
+        const i64 tb = it.t0 + (i64)c * kQ;
+        if (a.cu != nullptr && it.t1 - tb < kQ) {
+          // The last block of a packed sequence, in part: its rows only.
+          wait(bar->yS[s], c >> 1);
+          const int nv = (int)(it.t1 - tb);
+          T* y = static_cast<T*>(a.y) + it.batch * a.ys_b + tb * a.ys_t + h0 * a.ys_h;
+#pragma unroll 1
+          for (int e = yt; e < 2 * kQ * 8; e += 256) {
+            const int box = e >> 10, r = (e >> 3) & 127, un = e & 7;
+            const int col = (WIDE ? 64 * box : 0) + 8 * un;
+            if (r < nv && col < a.P && (WIDE || box < nh))
+              *reinterpret_cast<uint4*>(y + r * a.ys_t + (WIDE ? 0 : box * a.ys_h) + col) =
+                  *reinterpret_cast<const uint4*>(sm + kOffX + s * kTile + box * kBox + r * 128 + ((un ^ (r & 7)) << 4));
+          }
+        }
       }
     }
-  } else if (warp >= 12) {
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
     // ---------------- state ----------------
     const int q = warp & 3, hf = (warp - 12) >> 2;
     const int row = q * 32 + lane;                   // row of dS^T
@@ -617,18 +742,35 @@ __global__ void __launch_bounds__(kThreads, 1) scan_tc_kernel(const __grid_const
         const i64 h = h0 + hs;
         if (a.init) {
           const i64 o = it.seq * a.is_s + h * a.is_h + e0;
+          if (a.init_f32) {
 #pragma unroll
-          for (int j = 0; j < 64; ++j)
-            if (64 * hf + j < a.N)
-              S[j] = a.init_f32 ? static_cast<const float*>(a.init)[o + j] : Cvt<T>::f(static_cast<const T*>(a.init)[o + j]);
+            for (int j = 0; j < 16; ++j)
+              if (64 * hf + 4 * j < a.N) {
+                const float4 v = *reinterpret_cast<const float4*>(static_cast<const float*>(a.init) + o + 4 * j);
+                S[4 * j] = v.x, S[4 * j + 1] = v.y, S[4 * j + 2] = v.z, S[4 * j + 3] = v.w;
+              }
+          } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              if (64 * hf + 4 * j < a.N) {
+                const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const T*>(a.init) + o + 4 * j);
+                const float2 v0 = Pair<T>::unpack(v.x), v1 = Pair<T>::unpack(v.y);
+                S[4 * j] = v0.x, S[4 * j + 1] = v0.y, S[4 * j + 2] = v1.x, S[4 * j + 3] = v1.y;
+              }
+          }
         }
+#pragma unroll 1
         for (int r = 0; r < it.seg; ++r) {  // the earlier segments, in order
           const i64 slot = (it.first + r) * a.H + h;
           const float dc = ex2_approx(a.decay[slot]);
           const float* part = a.part + slot * a.P * a.N + e0;
 #pragma unroll
-          for (int j = 0; j < 64; ++j)
-            if (64 * hf + j < a.N) S[j] = fmaf(S[j], dc, part[j]);
+          for (int j = 0; j < 16; ++j)
+            if (64 * hf + 4 * j < a.N) {
+              const float4 v = *reinterpret_cast<const float4*>(part + 4 * j);
+              S[4 * j] = fmaf(S[4 * j], dc, v.x), S[4 * j + 1] = fmaf(S[4 * j + 1], dc, v.y);
+              S[4 * j + 2] = fmaf(S[4 * j + 2], dc, v.z), S[4 * j + 3] = fmaf(S[4 * j + 3], dc, v.w);
+            }
         }
       }
     }
@@ -647,21 +789,44 @@ __global__ void __launch_bounds__(kThreads, 1) scan_tc_kernel(const __grid_const
       fence_proxy_async_smem();
       warp_arrive(&bar->sR);
     };
-    if (!PART) put();
-    unsigned n = 0;      // slots of w X used
     float total = 0.f;   // base-2 log of the segment's decay
     const int xbox = q >> 1, xc = row & 63;
     constexpr bool kRowScale = std::is_same<T, __half>::value && TERMS > 1;
+    float dec = 1.f, unscale = 1.f;
+    // S = dec * S + dS of block c.
+    auto update = [&](unsigned c) {
+      wait(bar->dR, c);
+      tc_after();
+      if (hf < p.nb) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          uint32_t v[16];
+          tm_ld16(tmem + lanes + kColD + 64 * hf + 16 * k, v);
+          tm_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 16; j += 2) {
+            const float2 n = fma2(f2(S[16 * k + j], S[16 * k + j + 1]), f2(dec, dec),
+                                  mul2(f2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), f2(unscale, unscale)));
+            S[16 * k + j] = n.x;
+            S[16 * k + j + 1] = n.y;
+          }
+        }
+      }
+      tc_before();
+      warp_arrive(&bar->dF);
+    };
+#pragma unroll 1
     for (unsigned c = 0; c < (unsigned)nblk; ++c) {
       const unsigned s = c & 1;
-      CC1D_WAITW(fullX[s], c >> 1)
-      CC1D_WAITW(fullB[s], c >> 1)
+      wait(bar->fullX[s], c >> 1);
       unsigned char* xt = sm + kOffX + s * kTile;
       const i64 tb = it.t0 + (i64)c * kQ;
       if (a.cu != nullptr && it.t1 - tb < kQ) {
         // The rows behind the sequence's end belong to others, whatever they
         // hold: zeros keep it out of the sums.
+        wait(bar->fullB[s], c >> 1);
         const int nv = (int)(it.t1 - tb);
+#pragma unroll 1
         for (int e = nv * 8 + st; e < kQ * 8; e += 256) {
           const uint4 z = make_uint4(0u, 0u, 0u, 0u);
           reinterpret_cast<uint4*>(xt)[e] = z;
@@ -670,104 +835,82 @@ __global__ void __launch_bounds__(kThreads, 1) scan_tc_kernel(const __grid_const
         }
         fence_proxy_async_smem();
         warp_arrive(&bar->xSync);
-        CC1D_WAITW(xSync, 0)  // a sequence has one such block, its last
+        wait(bar->xSync, 0);  // a sequence has one such block, its last
       }
-      CC1D_WAITW(cumF[s], c >> 1)
+      wait(bar->cumF[s], c >> 1);
       const Cum& u = cum[s][hs];
       // x of token t in this thread's column.
       auto x_at = [&](int t) {
         return Cvt<T>::f(*reinterpret_cast<const T*>(xt + xbox * kBox + t * 128 + ((((xc >> 3) ^ (t & 7)) << 4) | ((xc & 7) << 1))));
       };
-      float scale = 1.f, unscale = u.unscale;
+      float scale = 1.f, next_unscale = u.unscale;
+      const float next_dec = u.dec;
       if (kRowScale) {
+        // The row's largest |w x|, of both its warps.
         float m = 0.f;
 #pragma unroll 8
         for (int k = 0; k < 64; ++k) {
-          const int t = 64 * (k >> 5) + 32 * hf + (k & 31);
+          const int t = 32 * (k >> 4) + 16 * hf + (k & 15);
           m = fmaxf(m, fabsf(u.w[t] * x_at(t)));
         }
         float* rm = reinterpret_cast<float*>(sm + kOffMax);
         rm[hf * kQ + row] = m;
         warp_arrive(&bar->mSync);
-        CC1D_WAITW(mSync, c)
+        wait(bar->mSync, c);
         const unsigned ex = max((__float_as_uint(fmaxf(rm[row], rm[kQ + row])) >> 23) & 255u, 15u);
         scale = __uint_as_float((268u - ex) << 23);  // the largest into [2^14, 2^15)
-        unscale = __uint_as_float((ex - 14u) << 23);
+        next_unscale = __uint_as_float((ex - 14u) << 23);
       }
-      bool ok = true;
 #pragma unroll 1
-      for (int half = 0; half < 2; ++half) {
-#pragma unroll
-        for (int k = 0; k < TERMS; ++k)
-          if (n + k >= 4) ok = ok && wait_or_abort(&bar->wF[(n + k) & 3], (((n + k) >> 2) - 1) & 1, abort_flag);
-        ok = __all_sync(kFull, ok);
-        if (!ok) break;
+      for (unsigned un = 0; un < 4; ++un) {
+        // The state of the block before, as soon as its last unit is through.
+        if (un == 1) {
+          if (c > 0) update(c - 1);
+          if (!PART) {
+            if (c > 0) wait(bar->iR, c - 1);  // inter has read the copy before
+            put();
+          }
+        }
+        const unsigned n = 4 * c + un;
+        if (n >= 2) wait(bar->wF[n & 1], (n >> 1) - 1);
         tc_after();
-        // This thread: tokens [64 half + 32 hf, + 32) of column p.
-#pragma unroll
-        for (int k16 = 0; k16 < 2; ++k16) {
-          const int t0 = 64 * half + 32 * hf + 16 * k16;
-          uint32_t o[TERMS][8];
+        const uint32_t at = tmem + lanes + kColW + (n & 1) * (16 * TERMS) + 8 * hf;
+        // This thread: 16 tokens of column p.
+#pragma unroll 1
+        for (int k8 = 0; k8 < 2; ++k8) {
+          const int t0 = 32 * un + 16 * hf + 8 * k8;
+          uint32_t o[TERMS][4];
           const float4* wp = reinterpret_cast<const float4*>(u.w + t0);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
+          for (int j = 0; j < 2; ++j) {
             const float4 w4 = wp[j];
-            const float wj[4] = {w4.x, w4.y, w4.z, w4.w};
-            float v[4];
+            float2 v[2] = {mul2(f2(w4.x, w4.y), f2(x_at(t0 + 4 * j), x_at(t0 + 4 * j + 1))),
+                           mul2(f2(w4.z, w4.w), f2(x_at(t0 + 4 * j + 2), x_at(t0 + 4 * j + 3)))};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              v[e] = wj[e] * x_at(t0 + 4 * j + e);
-              if (kRowScale) v[e] *= scale;
-            }
+            for (int e = 0; e < 2; ++e) {
+              if (kRowScale) v[e] = mul2(v[e], f2(scale, scale));
 #pragma unroll
-            for (int k = 0; k < TERMS; ++k) {
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const uint32_t w = Pair<T>::pack(f2(v[2 * e], v[2 * e + 1]));
-                o[k][2 * j + e] = w;
-                if (k + 1 < TERMS) {
-                  const float2 back = Pair<T>::unpack(w);
-                  v[2 * e] -= back.x;
-                  v[2 * e + 1] -= back.y;
-                }
-              }
+              for (int k = 0; k < TERMS; ++k) o[k][2 * j + e] = take_term<T, (TERMS > 1)>(v[e]);
             }
           }
 #pragma unroll
-          for (int k = 0; k < TERMS; ++k) tm_st8(tmem + lanes + kColW + ((n + k) & 3) * 32 + 16 * hf + 8 * k16, o[k]);
+          for (int k = 0; k < TERMS; ++k) tm_st4(at + 16 * k + 4 * k8, o[k]);
         }
         tm_st_wait();
         tc_before();
-        __syncwarp();
-        if (lane == 0) {
-          for (int k = 0; k < TERMS; ++k) mbar_arrive(&bar->wR[(n + k) & 3]);
-        }
-        n += TERMS;
+        warp_arrive(&bar->wR[n & 1]);
       }
-      if (!ok) break;
-      if (PART) warp_arrive(&bar->emptyX[s]);
-      const float dec = u.dec;
-      if (PART) total += u.tot[0] + u.tot[1] + u.tot[2] + u.tot[3];
+      if (PART) {
+        total += u.tot[0] + u.tot[1] + u.tot[2] + u.tot[3];
+        warp_arrive(&bar->emptyX[s]);
+      } else {
+        warp_arrive(&bar->xF[s]);
+      }
       warp_arrive(&bar->cumE[s]);
-      CC1D_WAITW(dR, c)
-      tc_after();
-      if (hf < p.nb) {
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          uint32_t v[32];
-          tm_ld32(tmem + lanes + kColD + 64 * hf + 32 * k, v);
-          tm_ld_wait();
-#pragma unroll
-          for (int j = 0; j < 32; ++j) S[32 * k + j] = fmaf(S[32 * k + j], dec, __uint_as_float(v[j]) * unscale);
-        }
-      }
-      tc_before();
-      warp_arrive(&bar->dF);
-      if (!PART && c + 1 < (unsigned)nblk) {
-        CC1D_WAITW(iR, c)  // inter has read the copy before
-        put();
-      }
+      dec = next_dec;
+      unscale = next_unscale;
     }
+    if (nblk > 0) update(nblk - 1);
     float* out = nullptr;
     if (live) {
       const i64 h = h0 + hs;
@@ -787,11 +930,10 @@ __global__ void __launch_bounds__(kThreads, 1) scan_tc_kernel(const __grid_const
           *reinterpret_cast<float4*>(out + 4 * j) = make_float4(S[4 * j], S[4 * j + 1], S[4 * j + 2], S[4 * j + 3]);
     }
   }
-#undef CC1D_WAIT1
-#undef CC1D_WAITW
   __syncwarp();
   tc_before();
   __syncthreads();
+  if (threadIdx.x == 0 && *(volatile int*)&bar->abort) atomicAdd(&g_cc1d_wait_timeouts, 1u);
   if (warp == 1) {
     tc_after();
     tm_dealloc(tmem);
@@ -876,6 +1018,7 @@ bool scan_tc_eligible(int dtype, const ScanArgs& a, i64 batch) {
          tile_ok(a.B, a.bs_n, a.G, a.bs_g, a.L, a.bs_t, batch, a.bs_b) &&
          tile_ok(a.C, a.cs_n, a.G, a.cs_g, a.L, a.cs_t, batch, a.cs_b) &&
          tile_ok(a.y, 1, a.H, a.ys_h, a.L, a.ys_t, batch, a.ys_b) &&
+         (a.init == nullptr || (reinterpret_cast<uintptr_t>(a.init) % 16 == 0 && a.is_s % 4 == 0 && a.is_h % 4 == 0)) &&
          (a.fin == nullptr || (reinterpret_cast<uintptr_t>(a.fin) % 16 == 0 && a.fs_s % 4 == 0 && a.fs_h % 4 == 0));
 }
 
@@ -889,6 +1032,7 @@ cudaError_t launch_scan_tc(int dtype, const ScanArgs& a, i64 batch, cudaStream_t
   t.nb = (int)ceil_div(a.N, 64);
   if (!make_map(&t.mx, bf, a.x, a.P, a.H, a.L, batch, a.xs_h, a.xs_t, a.xs_b) ||
       !make_map(&t.mb, bf, a.B, a.N, a.G, a.L, batch, a.bs_g, a.bs_t, a.bs_b) ||
+      !make_map(&t.my, bf, a.y, a.P, a.H, a.L, batch, a.ys_h, a.ys_t, a.ys_b) ||
       !make_map(&t.mc, bf, a.C, a.N, a.G, a.L, batch, a.cs_g, a.cs_t, a.cs_b))
     return cudaErrorInvalidValue;
   if (bf) return wide ? launch_all<__nv_bfloat16, true>(t, stream) : launch_all<__nv_bfloat16, false>(t, stream);
