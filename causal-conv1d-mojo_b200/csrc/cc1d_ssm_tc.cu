@@ -21,8 +21,9 @@
 //   exp(c_i - c_j) = exp(sum from j+1 to the end of j's sub-block)
 //                    * exp(whole sub-blocks between) * exp(sum up to i in its own),
 // a value per j, times a value per i and sub-block: 32 exponentials per row
-// instead of 128.  All factors are <= 1, so nothing overflows.  w_j sums from
-// the block's end backwards.  A step's a_t is held at -160 in base 2 (its
+// instead of 128.  All factors are <= 1, so nothing overflows.  w_j is such a
+// value per j, summed from the sub-block's end backwards, times one per
+// sub-block.  A step's a_t is held at -160 in base 2 (its
 // decay is 0 in fp32 from -150 on), which keeps the sums exact enough when
 // single steps forget everything.
 //
@@ -33,8 +34,8 @@
 // bf16 (24 bits) or two of fp16 (22 bits), so the states keep fp32 accuracy
 // (one bf16 term leaves a relative error of 1.7e-3, two 3e-6).  Without final
 // states one term is enough for y.  fp16 has few exponents: there w X is
-// scaled by a power of two, per row p to just under fp16's largest value (or
-// with one term per head to w < 1), which dS is scaled back by.
+// scaled by a power of two, per row p to just under fp16's largest value, which
+// dS is scaled back by.
 //
 // Roles (20 warps, one CTA per SM):
 //   warp 0       TMA: B and X in rings of two blocks, C in one buffer
@@ -43,8 +44,7 @@
 //   warp 2       issues dS: the chains of y and of the state meet only where
 //                one needs the other, and one issuer for both would make each
 //                wait for the other's barriers
-//   warp 3       step lengths and decay factors of the next block
-//   warps 4-11   tokens: thread = token row.  M from G, in place in TMEM (16
+//   warps 4-11   tokens: thread = token row.  Steps and decays of the next block;  M from G, in place in TMEM (16
 //                fp32 columns become 8 + 8 of pairs, one head each); scales inter by exp(c_i), so that intra accumulates
 //                onto it; y + D x over x in shared memory
 //   warps 12-19  state: thread = row p of S, half of n.  (w X)^T into TMEM,
@@ -87,29 +87,24 @@ constexpr unsigned kOffC = kOffX + 2 * kTile;
 constexpr unsigned kOffS = kOffC + kTile;
 constexpr unsigned kOffCum = kOffS + kTile;
 
-// Decay factors of one head in one block.
+// Steps and decays of one head in one block.
 struct Cum {
   float l[kQ];      // base-2 sum inside the sub-block, up to and with the token
   float d[kQ];      // step length
   float u[kQ];      // d * 2^(sum after the token inside its sub-block)
-  float w[kQ];      // d * 2^(sum after the token in the block) * scale
-  float e[kQ];      // 2^(sum up to and with the token in the block)
   float tot[4];     // sums of the sub-blocks
-  float dec;        // 2^(sum of the block)
-  float unscale;    // 1 / scale
-  float pad[2];
 };
 constexpr unsigned kOffMax = kOffCum + 2 * 2 * sizeof(Cum);  // fp16: largest |w x| per row, [half][128]
 constexpr unsigned kOffBar = kOffMax + 2 * kQ * 4;
 
 struct Bars {
   uint64_t fullB[2], fullX[2], fullC;
-  uint64_t emptyB[2], emptyX[2], emptyC;
-  uint64_t cumF[2], cumE[2];
+  uint64_t emptyB[2], emptyC;
+  uint64_t cumF[2];
   uint64_t gR, iR, pR, yR, yF;
   uint64_t wR[2], wF[2];
   uint64_t dR, dF, sR, end, endS;
-  uint64_t xF[2], yS[2];  // the state's warps have read x; y is in its place
+  uint64_t xF[2], yS[2];  // the state's warps have read x and the steps; y is in x's place
   uint64_t xSync, mSync;  // among the state warps
   uint32_t tmem;
   int abort;
@@ -177,9 +172,16 @@ __device__ __forceinline__ void tm_st8(uint32_t t, const uint32_t (&r)[8]) {
       "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(t)
       : "memory");
 }
-__device__ __forceinline__ void tm_st4(uint32_t t, const uint32_t (&r)[4]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%4], {%0, %1, %2, %3};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]),
-               "r"(r[3]), "r"(t)
+// Four 8x8 tiles of pairs (rows x 4 columns) into 16 lanes x 8 columns: lane
+// l's registers are row l / 4 and l / 4 + 8 of column l % 4, then of l % 4 + 4.
+__device__ __forceinline__ void tm_st_16x128(uint32_t t, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("tcgen05.st.sync.aligned.16x128b.x2.b32 [%0], {%1, %2, %3, %4};" ::"r"(t), "r"(a), "r"(b), "r"(c), "r"(d)
+               : "memory");
+}
+__device__ __forceinline__ void ldmatrix_t(uint32_t addr, uint32_t& a, uint32_t& b, uint32_t& c, uint32_t& d) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(a), "=r"(b), "=r"(c), "=r"(d)
+               : "r"(addr)
                : "memory");
 }
 __device__ __forceinline__ void tm_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
@@ -290,11 +292,9 @@ __global__ void __launch_bounds__(kThreads, 1) scan_tc_kernel(const __grid_const
       mbar_init(&bar->fullB[s], 1);
       mbar_init(&bar->fullX[s], 1);
       mbar_init(&bar->emptyB[s], PART ? 1 : 2);  // both issuers
-      mbar_init(&bar->emptyX[s], 8);
-      mbar_init(&bar->cumF[s], 1);
+      mbar_init(&bar->cumF[s], 8);
       mbar_init(&bar->xF[s], 8);
       mbar_init(&bar->yS[s], 8);
-      mbar_init(&bar->cumE[s], PART ? 8 : 16);
     }
     mbar_init(&bar->fullC, 1);
     mbar_init(&bar->emptyC, 1);
@@ -362,7 +362,7 @@ __global__ void __launch_bounds__(kThreads, 1) scan_tc_kernel(const __grid_const
         for (int k = 0; k < p.nb; ++k) tma_tile(sm + kOffB + s * kTile + k * kBox, &p.mb, &bar->fullB[s], 64 * k, g, t, b);
         if (c >= 2) {
           if (PART)
-            wait(bar->emptyX[s], (c >> 1) - 1);
+            wait(bar->xF[s], (c >> 1) - 1);
           else
             store(c - 2);
         }
@@ -491,114 +491,60 @@ __global__ void __launch_bounds__(kThreads, 1) scan_tc_kernel(const __grid_const
       if (lead) tc_commit(&bar->endS);
       wait(bar->endS, 0);
     }
-  } else {
-    // ---------------- steps and decays ----------------
-    const i64 o = it.batch * a.ds_b + h0 * a.ds_h;
-    constexpr int kH = WIDE ? 1 : 2;
-    const int es = a.dt_f32 ? 4 : (int)sizeof(T);
-    const char* dp = static_cast<const char*>(a.dt) + (o + (it.t0 + lane) * a.ds_t) * es;
-    const i64 hstep = a.ds_h * es, tstep = 32 * a.ds_t * es;
-    // dt of the lane's four tokens, both heads; the next block's are on their
-    // way while this one's are worked on.
-    auto load = [&](unsigned c, float (&d)[kH][4]) {
-      const i64 left = it.t1 - it.t0 - (i64)c * kQ - lane;
-#pragma unroll
-      for (int k = 0; k < kH; ++k) {
-        const char* q4 = dp + k * hstep;
-#pragma unroll
-        for (int q = 0; q < 4; ++q, q4 += tstep) {
-          d[k][q] = 0.f;
-          if (k < nh && left > 32 * q)
-            d[k][q] = a.dt_f32 ? *reinterpret_cast<const float*>(q4) : Cvt<T>::f(*reinterpret_cast<const T*>(q4));
-        }
-      }
-      dp += 4 * tstep;
-    };
-    float d[kH][4];
-    if (nblk > 0) load(0, d);
-#pragma unroll 1
-    for (unsigned c = 0; c < (unsigned)nblk; ++c) {
-      const unsigned s = c & 1;
-      if (c >= 2) wait(bar->cumE[s], (c >> 1) - 1);
-#pragma unroll
-      for (int k = 0; k < kH; ++k) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) cum[s][k].d[q * 32 + lane] = d[k][q];
-      }
-      if (c + 1 < (unsigned)nblk) load(c + 1, d);
-      const int left = (int)min(it.t1 - it.t0 - (i64)c * kQ, (i64)kQ) - lane;
-#pragma unroll 1
-      for (int k = 0; k < kH; ++k) {
-        Cum& u = cum[s][k];
-        const bool head = k < nh;
-        const float A2 = head ? a.A[h0 + k] * kLog2e : 0.f, bias = head && a.dt_bias ? a.dt_bias[h0 + k] : 0.f;
-        float l[4], r[4], tot[4];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          // Tokens behind the end, and a head that is not there: steps of length 0.
-          float d1 = u.d[q * 32 + lane] + bias;
-          d1 = !head || left <= 32 * q ? 0.f : a.softplus ? softplus_f(d1) : d1;
-          u.d[q * 32 + lane] = d1;
-          l[q] = r[q] = fmaxf(d1 * A2, -160.f);
-        }
-#pragma unroll
-        for (int sh = 1; sh < 32; sh <<= 1) {
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const float up = __shfl_up_sync(kFull, l[q], sh), dn = __shfl_down_sync(kFull, r[q], sh);
-            if (lane >= sh) l[q] += up;
-            if (lane + sh < 32) r[q] += dn;
-          }
-        }
-        float before[4], after[4];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          tot[q] = __shfl_sync(kFull, r[q], 0);
-          r[q] = __shfl_down_sync(kFull, r[q], 1);
-          if (lane == 31) r[q] = 0.f;
-        }
-        before[0] = 0.f, before[1] = tot[0], before[2] = tot[0] + tot[1], before[3] = before[2] + tot[2];
-        after[3] = 0.f, after[2] = tot[3], after[1] = tot[2] + tot[3], after[0] = tot[1] + after[1];
-        float w[4], big = 0.f;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int t = q * 32 + lane;
-          const float d1 = u.d[t];
-          u.l[t] = l[q];
-          u.u[t] = d1 * ex2_approx(r[q]);
-          w[q] = d1 * ex2_approx(r[q] + after[q]);
-          u.e[t] = ex2_approx(before[q] + l[q]);
-          big = fmaxf(big, fabsf(w[q]));
-        }
-        // fp16, one term: the largest weight into [1/2, 1), so that w x cannot overflow.
-        float scale = 1.f, unscale = 1.f;
-        if (std::is_same<T, __half>::value && TERMS == 1) {
-#pragma unroll
-          for (int sh = 16; sh > 0; sh >>= 1) big = fmaxf(big, __shfl_xor_sync(kFull, big, sh));
-          const int ex = min(max((int)((__float_as_uint(big) >> 23) & 255u), 27), 227);
-          scale = __uint_as_float((unsigned)(253 - ex) << 23);
-          unscale = __uint_as_float((unsigned)(ex + 1) << 23);
-        }
-#pragma unroll
-        for (int q = 0; q < 4; ++q) u.w[q * 32 + lane] = w[q] * scale;
-        if (lane < 4) u.tot[lane] = lane == 0 ? tot[0] : lane == 1 ? tot[1] : lane == 2 ? tot[2] : tot[3];
-        if (lane == 0) {
-          u.dec = ex2_approx(before[3] + tot[3]);
-          u.unscale = unscale;
-        }
-      }
-      warp_arrive(&bar->cumF[s]);
-    }
   }
   } else if (warp < 12) {
     // ---------------- tokens ----------------
-    if (!PART) {
-      const int q = warp & 3, hf = (warp - 4) >> 2;
-      const int row = q * 32 + lane;
-      const uint32_t lanes = (uint32_t)(q * 32) << 16;
-      const int hs = WIDE ? 0 : hf;  // head slot of this thread's y columns
-      const int yt = threadIdx.x - 128;
-      const float Dh = a.D && hs < nh ? a.D[h0 + hs] : 0.f;
+    const int q = warp & 3, hf = (warp - 4) >> 2;
+    const int row = q * 32 + lane;
+    const uint32_t lanes = (uint32_t)(q * 32) << 16;
+    const int hs = WIDE ? 0 : hf;  // head slot of this thread's y columns
+    const int yt = threadIdx.x - 128;
+    const float Dh = a.D && hs < nh ? a.D[h0 + hs] : 0.f;
+    // Steps and decays: a warp takes a sub-block of a head, a lane a token.
+    const bool cums = !WIDE || hf == 0;
+    const bool head = cums && hf < nh;
+    const float A2 = head ? a.A[h0 + hf] * kLog2e : 0.f, bias = head && a.dt_bias ? a.dt_bias[h0 + hf] : 0.f;
+    i64 dto = it.batch * a.ds_b + (h0 + hf) * a.ds_h + (it.t0 + row) * a.ds_t;
+    // dt of block c, asked for a block ahead and left as it is stored (a
+    // conversion here would wait for it); 0 where there is none.
+    auto raw_step = [&](unsigned c) {
+      uint32_t d = 0u;
+      if (head && it.t0 + (i64)c * kQ + row < it.t1)
+        d = a.dt_f32 ? static_cast<const uint32_t*>(a.dt)[dto] : static_cast<const uint16_t*>(a.dt)[dto];
+      dto += kQ * a.ds_t;
+      return d;
+    };
+    uint32_t raw = raw_step(0);
+    auto steps = [&](unsigned c) {
+      if (cums) {
+        Cum& u = cum[c & 1][hf];
+        // Tokens behind the end, and a head that is not there: steps of length 0.
+        float d = (a.dt_f32 ? __uint_as_float(raw) : Pair<T>::unpack(raw).x) + bias;
+        d = !head || it.t0 + (i64)c * kQ + row >= it.t1 ? 0.f : a.softplus ? softplus_f(d) : d;
+        if (c + 1 < (unsigned)nblk) raw = raw_step(c + 1);
+        float l = fmaxf(d * A2, -160.f), r = l;
+#pragma unroll
+        for (int sh = 1; sh < 32; sh <<= 1) {
+          const float up = __shfl_up_sync(kFull, l, sh), dn = __shfl_down_sync(kFull, r, sh);
+          if (lane >= sh) l += up;
+          if (lane + sh < 32) r += dn;
+        }
+        if (lane == 0) u.tot[q] = r;
+        r = __shfl_down_sync(kFull, r, 1);
+        u.l[row] = l;
+        u.d[row] = d;
+        u.u[row] = lane == 31 ? d : d * ex2_approx(r);
+      }
+      warp_arrive(&bar->cumF[c & 1]);
+    };
+    if (PART) {
+#pragma unroll 1
+      for (unsigned c = 0; c < (unsigned)nblk; ++c) {
+        if (c >= 2) wait(bar->xF[c & 1], (c >> 1) - 1);
+        steps(c);
+      }
+    } else {
+      if (nblk > 0) steps(0);
 #pragma unroll 1
       for (unsigned c = 0; c < (unsigned)nblk; ++c) {
         const unsigned s = c & 1;
@@ -609,77 +555,100 @@ __global__ void __launch_bounds__(kThreads, 1) scan_tc_kernel(const __grid_const
         // fp32 columns become 8 + 8 columns of 16-bit pairs, one head each.
         constexpr int kH = WIDE ? 1 : 2;
         const uint32_t atG = tmem + lanes + kColG + 16 * hf;
+        // While G runs: the row's own sum, its decay from the start of the
+        // block (for inter), from the ends of the sub-blocks before its own.
+        float l[kH], f[kH][3], e = 0.f;
+#pragma unroll
+        for (int k = 0; k < kH; ++k) {
+          float sum = l[k] = cu[k].l[row];
+#pragma unroll
+          for (int b = 2; b >= 0; --b) {
+            f[k][b] = ex2_approx(sum);
+            if (b < q) sum += cu[k].tot[b];
+          }
+          if (k == hs) e = ex2_approx(sum);
+        }
         wait(bar->gR, c);
         tc_after();
-        uint32_t v[16];
-        tm_ld16(atG + 32 * q, v);
-        tm_ld_wait();
-        const int last = lane - 16 * hf;  // last unmasked column of the row's own sub-block
-#pragma unroll 1
-        for (int k = 0; k < kH; ++k) {
-          const Cum& u = cu[k];
-          const float l = u.l[row];
-          const float4* lp = reinterpret_cast<const float4*>(u.l + 32 * q + 16 * hf);
-          const float4* dp = reinterpret_cast<const float4*>(u.d + 32 * q + 16 * hf);
-          uint32_t o[8];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float4 l4 = lp[j], d4 = dp[j];
-            const float m0 = 4 * j + 0 <= last ? __uint_as_float(v[4 * j + 0]) * (ex2_approx(l - l4.x) * d4.x) : 0.f;
-            const float m1 = 4 * j + 1 <= last ? __uint_as_float(v[4 * j + 1]) * (ex2_approx(l - l4.y) * d4.y) : 0.f;
-            const float m2 = 4 * j + 2 <= last ? __uint_as_float(v[4 * j + 2]) * (ex2_approx(l - l4.z) * d4.z) : 0.f;
-            const float m3 = 4 * j + 3 <= last ? __uint_as_float(v[4 * j + 3]) * (ex2_approx(l - l4.w) * d4.w) : 0.f;
-            o[2 * j] = Pair<T>::pack(f2(m0, m1));
-            o[2 * j + 1] = Pair<T>::pack(f2(m2, m3));
-          }
-          tm_st8(atG + 32 * q + 8 * k, o);
-        }
-#pragma unroll 1
-        for (int b = q - 1; b >= 0; --b) {
-          tm_ld16(atG + 32 * b, v);
+        {
+          uint32_t v[16];
+          tm_ld16(atG + 32 * q, v);
           tm_ld_wait();
-#pragma unroll 1
+          const int last = lane - 16 * hf;  // last unmasked column of the row's own sub-block
+#pragma unroll
           for (int k = 0; k < kH; ++k) {
-            const Cum& u = cu[k];
-            // Decay from the end of sub-block b to the row.
-            float f = u.l[row];
-            for (int m = b + 1; m < q; ++m) f += u.tot[m];
-            f = ex2_approx(f);
-            const float2 ff = f2(f, f);
-            const float4* up = reinterpret_cast<const float4*>(u.u + 32 * b + 16 * hf);
+            const float4* lp = reinterpret_cast<const float4*>(cu[k].l + 32 * q + 16 * hf);
+            const float4* dp = reinterpret_cast<const float4*>(cu[k].d + 32 * q + 16 * hf);
             uint32_t o[8];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              const float4 w4 = up[j];
-              o[2 * j] = Pair<T>::pack(mul2(mul2(f2(__uint_as_float(v[4 * j]), __uint_as_float(v[4 * j + 1])), f2(w4.x, w4.y)), ff));
-              o[2 * j + 1] = Pair<T>::pack(mul2(mul2(f2(__uint_as_float(v[4 * j + 2]), __uint_as_float(v[4 * j + 3])), f2(w4.z, w4.w)), ff));
+              const float4 l4 = lp[j], d4 = dp[j];
+              const float m0 = 4 * j + 0 <= last ? __uint_as_float(v[4 * j + 0]) * (ex2_approx(l[k] - l4.x) * d4.x) : 0.f;
+              const float m1 = 4 * j + 1 <= last ? __uint_as_float(v[4 * j + 1]) * (ex2_approx(l[k] - l4.y) * d4.y) : 0.f;
+              const float m2 = 4 * j + 2 <= last ? __uint_as_float(v[4 * j + 2]) * (ex2_approx(l[k] - l4.z) * d4.z) : 0.f;
+              const float m3 = 4 * j + 3 <= last ? __uint_as_float(v[4 * j + 3]) * (ex2_approx(l[k] - l4.w) * d4.w) : 0.f;
+              o[2 * j] = Pair<T>::pack(f2(m0, m1));
+              o[2 * j + 1] = Pair<T>::pack(f2(m2, m3));
             }
-            tm_st8(atG + 32 * b + 8 * k, o);
+            tm_st8(atG + 32 * q + 8 * k, o);
           }
         }
 #pragma unroll
-        for (int j = 0; j < 16; ++j) v[j] = 0u;
-#pragma unroll 1
-        for (int b = q + 1; b < 4; ++b) tm_st16(atG + 32 * b, v);
-        // inter times exp(c_i), in place.
-        wait(bar->iR, c);
-        tc_after();
-        {
-          const float e = cu[hs].e[row];
-#pragma unroll 1
-          for (int k = 0; k < 4; ++k) {
-            const uint32_t at = tmem + lanes + kColY + 64 * hf + 16 * k;
-            tm_ld16(at, v);
+        for (int b = 0; b < 3; ++b) {
+          if (b < q) {
+            uint32_t v[16];
+            tm_ld16(atG + 32 * b, v);
             tm_ld_wait();
 #pragma unroll
-            for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) * e);
-            tm_st16(at, v);
+            for (int k = 0; k < kH; ++k) {
+              const float2 ff = f2(f[k][b], f[k][b]);
+              const float4* up = reinterpret_cast<const float4*>(cu[k].u + 32 * b + 16 * hf);
+              uint32_t o[8];
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const float4 w4 = up[j];
+                o[2 * j] = Pair<T>::pack(mul2(mul2(f2(__uint_as_float(v[4 * j]), __uint_as_float(v[4 * j + 1])), f2(w4.x, w4.y)), ff));
+                o[2 * j + 1] = Pair<T>::pack(mul2(mul2(f2(__uint_as_float(v[4 * j + 2]), __uint_as_float(v[4 * j + 3])), f2(w4.z, w4.w)), ff));
+              }
+              tm_st8(atG + 32 * b + 8 * k, o);
+            }
+          }
+        }
+        {
+          uint32_t v[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) v[j] = 0u;
+#pragma unroll 1
+          for (int b = q + 1; b < 4; ++b) tm_st16(atG + 32 * b, v);
+        }
+        // inter times exp(c_i), in place.
+        const uint32_t atY = tmem + lanes + kColY + 64 * hf;
+        wait(bar->iR, c);
+        tc_after();
+#pragma unroll 1
+        for (int k = 0; k < 2; ++k) {
+          uint32_t v[2][16];
+          tm_ld16(atY + 32 * k, v[0]);
+          tm_ld16(atY + 32 * k + 16, v[1]);
+          tm_ld_wait();
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int j = 0; j < 16; j += 2) {
+              const float2 w = mul2(f2(__uint_as_float(v[h][j]), __uint_as_float(v[h][j + 1])), f2(e, e));
+              v[h][j] = __float_as_uint(w.x);
+              v[h][j + 1] = __float_as_uint(w.y);
+            }
+            tm_st16(atY + 32 * k + 16 * h, v[h]);
           }
         }
         tm_st_wait();
         tc_before();
         warp_arrive(&bar->pR);
-        warp_arrive(&bar->cumE[s]);
+        // The next block's steps, while intra runs.  Their stage is free: the
+        // tokens' warps have read it before pR, the state's before xF, of the
+        // block before.
+        if (c + 1 < (unsigned)nblk) steps(c + 1);
         // y + D x, over x.
         wait(bar->yR, c);
         wait(bar->xF[s], c >> 1);
@@ -687,24 +656,31 @@ __global__ void __launch_bounds__(kThreads, 1) scan_tc_kernel(const __grid_const
         uint4* xr = reinterpret_cast<uint4*>(sm + kOffX + s * kTile + hf * kBox + row * 128);
         const int sw = row & 7;
 #pragma unroll 1
-        for (int k = 0; k < 4; ++k) {
-          tm_ld16(tmem + lanes + kColY + 64 * hf + 16 * k, v);
+        for (int k = 0; k < 2; ++k) {
+          uint32_t v[2][16];
+          tm_ld16(atY + 32 * k, v[0]);
+          tm_ld16(atY + 32 * k + 16, v[1]);
+          uint4 x4[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) x4[j] = xr[(4 * k + j) ^ sw];
           tm_ld_wait();
+          if (k == 1) {
+            tc_before();
+            warp_arrive(&bar->yF);  // inter of the next block may come
+          }
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            uint4 w = xr[(2 * k + j) ^ sw];
-            uint32_t* wp = &w.x;
+          for (int j = 0; j < 4; ++j) {
+            uint32_t* wp = &x4[j].x;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float2 xv = Pair<T>::unpack(wp[e]);
-              wp[e] = Pair<T>::pack(fma2(f2(Dh, Dh), xv, f2(__uint_as_float(v[8 * j + 2 * e]), __uint_as_float(v[8 * j + 2 * e + 1]))));
+            for (int h = 0; h < 4; ++h) {
+              const int o = 8 * (j & 1) + 2 * h;
+              wp[h] = Pair<T>::pack(fma2(f2(Dh, Dh), Pair<T>::unpack(wp[h]),
+                                         f2(__uint_as_float(v[j >> 1][o]), __uint_as_float(v[j >> 1][o + 1]))));
             }
-            xr[(2 * k + j) ^ sw] = w;
+            xr[(4 * k + j) ^ sw] = x4[j];
           }
         }
-        tc_before();
         fence_proxy_async_smem();
-        warp_arrive(&bar->yF);
         warp_arrive(&bar->yS[s]);
         const i64 tb = it.t0 + (i64)c * kQ;
         if (a.cu != nullptr && it.t1 - tb < kQ) {
@@ -774,46 +750,67 @@ __global__ void __launch_bounds__(kThreads, 1) scan_tc_kernel(const __grid_const
         }
       }
     }
-    // 16-bit copy of the state for inter: row p, this thread's half of n.
-    auto put = [&]() {
-      uint4* sr = reinterpret_cast<uint4*>(sm + kOffS + hf * kBox + row * 128);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        uint4 w;
-        w.x = Pair<T>::pack(f2(S[8 * j], S[8 * j + 1]));
-        w.y = Pair<T>::pack(f2(S[8 * j + 2], S[8 * j + 3]));
-        w.z = Pair<T>::pack(f2(S[8 * j + 4], S[8 * j + 5]));
-        w.w = Pair<T>::pack(f2(S[8 * j + 6], S[8 * j + 7]));
-        sr[j ^ (row & 7)] = w;
-      }
-      fence_proxy_async_smem();
-      warp_arrive(&bar->sR);
-    };
     float total = 0.f;   // base-2 log of the segment's decay
-    const int xbox = q >> 1, xc = row & 63;
-    constexpr bool kRowScale = std::is_same<T, __half>::value && TERMS > 1;
+    constexpr bool kRowScale = std::is_same<T, __half>::value;
     float dec = 1.f, unscale = 1.f;
-    // S = dec * S + dS of block c.
-    auto update = [&](unsigned c) {
-      wait(bar->dR, c);
-      tc_after();
-      if (hf < p.nb) {
+    // S = dec * S + dS of block c - 1 (c > 0), and with `copy` the 16-bit copy
+    // of S for inter: row p, this thread's half of n.
+    auto advance = [&](unsigned c, bool copy) {
+      if (c > 0) {
+        wait(bar->dR, c - 1);
+        if (copy) wait(bar->iR, c - 1);  // inter has read the copy before
+        tc_after();
+      }
+      uint4* sr = reinterpret_cast<uint4*>(sm + kOffS + hf * kBox + row * 128);
+      const float2 dd = f2(dec, dec), uu = f2(unscale, unscale);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          uint32_t v[16];
-          tm_ld16(tmem + lanes + kColD + 64 * hf + 16 * k, v);
+      for (int k = 0; k < 2; ++k) {
+        if (c > 0 && hf < p.nb) {
+          uint32_t v[2][16];
+          tm_ld16(tmem + lanes + kColD + 64 * hf + 32 * k, v[0]);
+          tm_ld16(tmem + lanes + kColD + 64 * hf + 32 * k + 16, v[1]);
           tm_ld_wait();
 #pragma unroll
-          for (int j = 0; j < 16; j += 2) {
-            const float2 n = fma2(f2(S[16 * k + j], S[16 * k + j + 1]), f2(dec, dec),
-                                  mul2(f2(__uint_as_float(v[j]), __uint_as_float(v[j + 1])), f2(unscale, unscale)));
-            S[16 * k + j] = n.x;
-            S[16 * k + j + 1] = n.y;
+          for (int j = 0; j < 32; j += 2) {
+            const float2 n = fma2(f2(S[32 * k + j], S[32 * k + j + 1]), dd,
+                                  mul2(f2(__uint_as_float(v[j >> 4][j & 15]), __uint_as_float(v[j >> 4][(j & 15) + 1])), uu));
+            S[32 * k + j] = n.x;
+            S[32 * k + j + 1] = n.y;
+          }
+        }
+        if (copy) {
+#pragma unroll
+          for (int j = 4 * k; j < 4 * k + 4; ++j) {
+            uint4 w;
+            w.x = Pair<T>::pack(f2(S[8 * j], S[8 * j + 1]));
+            w.y = Pair<T>::pack(f2(S[8 * j + 2], S[8 * j + 3]));
+            w.z = Pair<T>::pack(f2(S[8 * j + 4], S[8 * j + 5]));
+            w.w = Pair<T>::pack(f2(S[8 * j + 6], S[8 * j + 7]));
+            sr[j ^ (row & 7)] = w;
           }
         }
       }
-      tc_before();
-      warp_arrive(&bar->dF);
+      if (c > 0) {
+        tc_before();
+        warp_arrive(&bar->dF);
+      }
+      if (copy) {
+        fence_proxy_async_smem();
+        warp_arrive(&bar->sR);
+      }
+    };
+    // x for w X comes transposed out of shared memory (ldmatrix), as lane l's
+    // columns p = l / 4 (+ 8, 16, 24) and tokens 2 (l % 4), + 1 of eight; the
+    // 16x128b stores put that into TMEM as rows p and columns of token pairs.
+    // Of each unit of 32 tokens this warp does 16: matrices of 8 tokens by 8
+    // columns in the order (first 8 tokens, second 8) x (8 columns, next 8).
+    const uint32_t xrow = smem_u32(sm) + kOffX + (q >> 1) * kBox + (16 * hf + ((lane >> 4) << 3) + (lane & 7)) * 128;
+    const uint32_t xcol0 = (((q & 1) * 4 + ((lane >> 3) & 1)) ^ (lane & 7)) << 4, xcol1 = xcol0 ^ (2 << 4);
+    const int wt = 16 * hf + 2 * (lane & 3);  // this lane's first token of a unit
+    auto load_x = [&](unsigned s, unsigned un, uint32_t (&x)[8]) {
+      const uint32_t at = xrow + s * kTile + un * (32 * 128);
+      ldmatrix_t(at + xcol0, x[0], x[1], x[2], x[3]);
+      ldmatrix_t(at + xcol1, x[4], x[5], x[6], x[7]);
     };
 #pragma unroll 1
     for (unsigned c = 0; c < (unsigned)nblk; ++c) {
@@ -839,78 +836,77 @@ __global__ void __launch_bounds__(kThreads, 1) scan_tc_kernel(const __grid_const
       }
       wait(bar->cumF[s], c >> 1);
       const Cum& u = cum[s][hs];
-      // x of token t in this thread's column.
-      auto x_at = [&](int t) {
-        return Cvt<T>::f(*reinterpret_cast<const T*>(xt + xbox * kBox + t * 128 + ((((xc >> 3) ^ (t & 7)) << 4) | ((xc & 7) << 1))));
-      };
-      float scale = 1.f, next_unscale = u.unscale;
-      const float next_dec = u.dec;
+      const float* uw = u.u + wt;
+      // Decay from the end of each sub-block to the block's end, of the whole block.
+      const float after2 = u.tot[3], after1 = u.tot[2] + after2, after0 = u.tot[1] + after1;
+      const float g0 = ex2_approx(after0), g1 = ex2_approx(after1), g2 = ex2_approx(after2);
+      uint32_t x[8];
+      float scale[4] = {1.f, 1.f, 1.f, 1.f}, next_unscale = 1.f;
+      const float next_dec = ex2_approx(u.tot[0] + after0);
       if (kRowScale) {
-        // The row's largest |w x|, of both its warps.
-        float m = 0.f;
-#pragma unroll 8
-        for (int k = 0; k < 64; ++k) {
-          const int t = 32 * (k >> 4) + 16 * hf + (k & 15);
-          m = fmaxf(m, fabsf(u.w[t] * x_at(t)));
+        // The largest |w x| of each row, of both its warps.
+        float m[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+        for (unsigned un = 0; un < 4; ++un) {
+          load_x(s, un, x);
+          const float g = un == 0 ? g0 : un == 1 ? g1 : un == 2 ? g2 : 1.f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float2 w = *reinterpret_cast<const float2*>(uw + 32 * un + 4 * (i & 2));
+            const float2 v = mul2(mul2(w, f2(g, g)), Pair<T>::unpack(x[i]));
+            m[2 * (i >> 2) + (i & 1)] = fmaxf(m[2 * (i >> 2) + (i & 1)], fmaxf(fabsf(v.x), fabsf(v.y)));
+          }
         }
         float* rm = reinterpret_cast<float*>(sm + kOffMax);
-        rm[hf * kQ + row] = m;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          m[i] = fmaxf(m[i], __shfl_xor_sync(kFull, m[i], 1));
+          m[i] = fmaxf(m[i], __shfl_xor_sync(kFull, m[i], 2));
+          if ((lane & 3) == 0) rm[hf * kQ + q * 32 + 8 * i + (lane >> 2)] = m[i];
+        }
         warp_arrive(&bar->mSync);
         wait(bar->mSync, c);
-        const unsigned ex = max((__float_as_uint(fmaxf(rm[row], rm[kQ + row])) >> 23) & 255u, 15u);
-        scale = __uint_as_float((268u - ex) << 23);  // the largest into [2^14, 2^15)
-        next_unscale = __uint_as_float((ex - 14u) << 23);
+        auto exponent = [&](int r) { return max((__float_as_uint(fmaxf(rm[r], rm[kQ + r])) >> 23) & 255u, 15u); };
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          scale[i] = __uint_as_float((268u - exponent(q * 32 + 8 * i + (lane >> 2))) << 23);  // the largest into [2^14, 2^15)
+        next_unscale = __uint_as_float((exponent(row) - 14u) << 23);
       }
 #pragma unroll 1
       for (unsigned un = 0; un < 4; ++un) {
         // The state of the block before, as soon as its last unit is through.
-        if (un == 1) {
-          if (c > 0) update(c - 1);
-          if (!PART) {
-            if (c > 0) wait(bar->iR, c - 1);  // inter has read the copy before
-            put();
-          }
-        }
+        if (un == 1) advance(c, !PART);
         const unsigned n = 4 * c + un;
+        load_x(s, un, x);
+        const float g = un == 0 ? g0 : un == 1 ? g1 : un == 2 ? g2 : 1.f;
+        const float2 w0 = mul2(*reinterpret_cast<const float2*>(uw + 32 * un), f2(g, g));
+        const float2 w1 = mul2(*reinterpret_cast<const float2*>(uw + 32 * un + 8), f2(g, g));
         if (n >= 2) wait(bar->wF[n & 1], (n >> 1) - 1);
         tc_after();
+        uint32_t o[TERMS][8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          float2 v = mul2((i & 2) ? w1 : w0, Pair<T>::unpack(x[i]));
+          if (kRowScale) v = mul2(v, f2(scale[2 * (i >> 2) + (i & 1)], scale[2 * (i >> 2) + (i & 1)]));
+#pragma unroll
+          for (int k = 0; k < TERMS; ++k) o[k][i] = take_term<T, (TERMS > 1)>(v);
+        }
         const uint32_t at = tmem + lanes + kColW + (n & 1) * (16 * TERMS) + 8 * hf;
-        // This thread: 16 tokens of column p.
-#pragma unroll 1
-        for (int k8 = 0; k8 < 2; ++k8) {
-          const int t0 = 32 * un + 16 * hf + 8 * k8;
-          uint32_t o[TERMS][4];
-          const float4* wp = reinterpret_cast<const float4*>(u.w + t0);
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const float4 w4 = wp[j];
-            float2 v[2] = {mul2(f2(w4.x, w4.y), f2(x_at(t0 + 4 * j), x_at(t0 + 4 * j + 1))),
-                           mul2(f2(w4.z, w4.w), f2(x_at(t0 + 4 * j + 2), x_at(t0 + 4 * j + 3)))};
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              if (kRowScale) v[e] = mul2(v[e], f2(scale, scale));
-#pragma unroll
-              for (int k = 0; k < TERMS; ++k) o[k][2 * j + e] = take_term<T, (TERMS > 1)>(v[e]);
-            }
-          }
-#pragma unroll
-          for (int k = 0; k < TERMS; ++k) tm_st4(at + 16 * k + 4 * k8, o[k]);
+        for (int k = 0; k < TERMS; ++k) {
+          tm_st_16x128(at + 16 * k, o[k][0], o[k][1], o[k][2], o[k][3]);
+          tm_st_16x128(at + 16 * k + (16u << 16), o[k][4], o[k][5], o[k][6], o[k][7]);
         }
         tm_st_wait();
         tc_before();
         warp_arrive(&bar->wR[n & 1]);
       }
-      if (PART) {
-        total += u.tot[0] + u.tot[1] + u.tot[2] + u.tot[3];
-        warp_arrive(&bar->emptyX[s]);
-      } else {
-        warp_arrive(&bar->xF[s]);
-      }
-      warp_arrive(&bar->cumE[s]);
+      if (PART) total += u.tot[0] + after0;
+      warp_arrive(&bar->xF[s]);  // x and the steps have been read
       dec = next_dec;
       unscale = next_unscale;
     }
-    if (nblk > 0) update(nblk - 1);
+    if (nblk > 0) advance(nblk, false);
     float* out = nullptr;
     if (live) {
       const i64 h = h0 + hs;
