@@ -324,11 +324,11 @@ __global__ void __launch_bounds__(kThreads, 1) scan_tc_kernel(const __grid_const
   const uint32_t tmem = bar->tmem;
   auto wait = [&](uint64_t& b, unsigned phase) { wait_for(&b, phase & 1, &bar->abort); };
 
-  // Registers: 96 a thread at launch (61440 in all); the state's warps take
-  // over what the first four do not need (4 * 32 * 64 + 8 * 32 * 96 +
-  // 8 * 32 * 112 = 61440).
+  // Registers: 96 a thread at launch (61440 in all); the other warps take over
+  // what the first four do not need (4 * 32 * 48 + 8 * 32 * 104 + 8 * 32 * 112
+  // = 61440).
   if (warp < 4) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
   if (warp == 0) {
     // ---------------- TMA ----------------
     if (lane == 0) {
@@ -493,6 +493,7 @@ __global__ void __launch_bounds__(kThreads, 1) scan_tc_kernel(const __grid_const
     }
   }
   } else if (warp < 12) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
     // ---------------- tokens ----------------
     const int q = warp & 3, hf = (warp - 4) >> 2;
     const int row = q * 32 + lane;
