@@ -42,8 +42,9 @@ class _GatedNormFn(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
+        if torch.is_grad_enabled():
+            raise RuntimeError("gated_norm_fn has no second derivative (backward with create_graph=True)")
         x, z, w, b, mean, rstd = ctx.saved_tensors
         eps, group_size, layer, gate_first = ctx.how
         dy = _rows(dy)

@@ -398,6 +398,8 @@ int cc1d_device_status(unsigned* wait_timeouts) {
   if (e != cudaSuccess) return cuda_fail(e, "cc1d_device_status");
   e = read_scan_wait_timeouts(wait_timeouts);
   if (e != cudaSuccess) return cuda_fail(e, "cc1d_device_status");
+  e = read_norm_wait_timeouts(wait_timeouts);
+  if (e != cudaSuccess) return cuda_fail(e, "cc1d_device_status");
   return ok();
 }
 

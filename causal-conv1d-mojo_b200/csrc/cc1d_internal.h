@@ -153,8 +153,9 @@ cudaError_t launch_finalize_peer(int dtype, int width, const PeerFinalizeArgs& p
 cudaError_t read_peer_timeouts(unsigned* count);
 // Blocks of the fused in_proj + conv kernel that gave up on a bounded wait.
 cudaError_t read_fused_aborts(unsigned* count);
-// Bounded waits of the tensor-core scan that gave up.
+// Bounded waits of the tensor-core scan and of the norm that gave up.
 cudaError_t read_scan_wait_timeouts(unsigned* count);
+cudaError_t read_norm_wait_timeouts(unsigned* count);
 
 // Records a message for cc1d_last_error() and returns `code` (for entry
 // points defined outside cc1d_abi.cu).

@@ -17,6 +17,7 @@
 
 #include "cc1d.h"
 #include "cc1d_dispatch.cuh"
+#include "cc1d_tma.cuh"
 
 namespace cc1d {
 
@@ -47,6 +48,24 @@ __device__ __forceinline__ float param(const void* p, i64 i, int f32) {
   return f32 ? static_cast<const float*>(p)[i] : Cvt<T>::f(static_cast<const T*>(p)[i]);
 }
 
+// V adjacent ones, by 16-byte loads (V > 1: the plan has checked the alignment).
+template <typename T, int V>
+__device__ __forceinline__ void load_params(const void* p, i64 i, int f32, float (&o)[V]) {
+  if constexpr (V == 1) {
+    o[0] = param<T>(p, i, f32);
+  } else if (f32) {
+#pragma unroll
+    for (int j = 0; j < V; j += 4) {
+      const float4 v = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p) + i + j));
+      o[j] = v.x, o[j + 1] = v.y, o[j + 2] = v.z, o[j + 3] = v.w;
+    }
+  } else {
+    const Pack<T, V> pk = ld_pack<T, V>(static_cast<const T*>(p) + i);
+#pragma unroll
+    for (int j = 0; j < V; ++j) o[j] = Cvt<T>::f(pk.v[j]);
+  }
+}
+
 // Sums of two values over a team: WARPS == 0, a warp; else the whole block,
 // through shared memory (two buffers in turn, so one barrier per sum).
 __device__ __forceinline__ float2 team_sum(float2 v, bool block, float2* buf, int nw) {
@@ -66,6 +85,22 @@ __device__ __forceinline__ float2 team_sum(float2 v, bool block, float2* buf, in
     v.y += __shfl_xor_sync(kFull, v.y, o);
   }
   return v;
+}
+
+// One value, the warps' parts added up by every thread itself.
+__device__ __forceinline__ float team_sum(float v, bool block, float* buf, int nw) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
+  if (!block) return v;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (lane == 0) buf[warp] = v;
+  __syncthreads();
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i = 0; i < nw; i += 4) {  // the buffer is 0 behind the last warp's part
+    const float4 p = *reinterpret_cast<const float4*>(buf + i);
+    sum.x += p.x, sum.y += p.y, sum.z += p.z, sum.w += p.w;
+  }
+  return (sum.x + sum.y) + (sum.z + sum.w);
 }
 
 // Where a thread's values lie: V adjacent columns at (k * team + t) * V, k < K.
@@ -92,12 +127,104 @@ __device__ __forceinline__ void store_cols(void* base, i64 off, const float (&o)
   st_pack<T, V>(static_cast<T*>(base) + off, pk);
 }
 
+// ---- rows through shared memory ----
+// With more than a few rows per block, each row's arrays come by bulk copies
+// into a ring of stages: a block then has the next rows' bytes on their way
+// without holding them in registers.  A stage is free again at the barrier of
+// its row's first sum, by when every thread has its values in registers.
+struct Ring {
+  unsigned char* base;
+  uint64_t* full;
+  int stages;
+  unsigned bytes;      // of one array's row
+  unsigned stage;      // of a stage
+};
+
+// A stage and its phase, counted along (the number of stages is no constant).
+struct RingAt {
+  unsigned s = 0, phase = 0;
+  __device__ __forceinline__ void next(int stages) {
+    if (++s == (unsigned)stages) s = 0, phase ^= 1;
+  }
+};
+
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, unsigned bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+// The group's weight (and bias) into shared memory, once per block: a block
+// reads them with every row, and with the ring next to it the L1 cache is too
+// small to keep them.
+template <typename T>
+__device__ __forceinline__ unsigned char* stage_params(const NormArgs& a, i64 c0, unsigned char* to) {
+  const int es = a.w_f32 ? 4 : (int)sizeof(T);
+  const int n16 = a.gs * es / 16;
+  const uint4* w = reinterpret_cast<const uint4*>(static_cast<const char*>(a.w) + c0 * es);
+  const uint4* b = a.b ? reinterpret_cast<const uint4*>(static_cast<const char*>(a.b) + c0 * es) : nullptr;
+  uint4* o = reinterpret_cast<uint4*>(to);
+  for (int i = threadIdx.x; i < n16; i += blockDim.x) {
+    o[i] = __ldg(w + i);
+    if (b) o[n16 + i] = __ldg(b + i);
+  }
+  return to + a.gs * es;  // the bias
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void smem_params(const unsigned char* p, int c, int f32, float (&o)[V]) {
+  if (f32) {
+#pragma unroll
+    for (int j = 0; j < V; j += 4) {
+      const float4 v = *reinterpret_cast<const float4*>(p + (c + j) * 4);
+      o[j] = v.x, o[j + 1] = v.y, o[j + 2] = v.z, o[j + 3] = v.w;
+    }
+  } else {
+    Pack<T, V> pk;
+    pk.raw = *reinterpret_cast<const typename Pack<T, V>::Raw*>(p + c * sizeof(T));
+#pragma unroll
+    for (int j = 0; j < V; ++j) o[j] = Cvt<T>::f(pk.v[j]);
+  }
+}
+
+template <int ARRAYS>
+__device__ __forceinline__ void ring_fill(const Ring& r, unsigned s, const void* const (&src)[ARRAYS]) {
+  mbar_arrive_expect_tx(&r.full[s], r.bytes * ARRAYS);
+#pragma unroll
+  for (int i = 0; i < ARRAYS; ++i) bulk_load(r.base + s * r.stage + i * r.bytes, src[i], r.bytes, &r.full[s]);
+}
+
+__device__ __forceinline__ Ring ring_make(unsigned char* smem, int stages, unsigned bytes, int arrays) {
+  Ring r{smem + 128, reinterpret_cast<uint64_t*>(smem), stages, bytes, bytes * arrays};
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < stages; ++s) mbar_init(&r.full[s], 1);
+    fence_mbar_init();
+  }
+  __syncthreads();
+  return r;
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void smem_cols(const unsigned char* row, int c, bool ok, float (&o)[V]) {
+  Pack<T, V> pk;
+  if (ok) {
+    pk.raw = *reinterpret_cast<const typename Pack<T, V>::Raw*>(row + c * sizeof(T));
+#pragma unroll
+    for (int j = 0; j < V; ++j) o[j] = Cvt<T>::f(pk.v[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) o[j] = 0.f;
+  }
+}
+
 // ---- forward ----
 // Team: one warp (several per block) when a group fits 32 * K * V columns,
-// else the block.
-template <typename T, int V, int K, bool GATE>
-__global__ void __launch_bounds__(512) norm_fwd_kernel(const __grid_constant__ NormArgs a, int warp_teams) {
-  __shared__ float2 buf[2][32];
+// else the block.  RING: block teams only.
+template <typename T, int V, int K, bool GATE, bool RING>
+__global__ void __launch_bounds__(512, RING ? 2 : 1) norm_fwd_kernel(const __grid_constant__ NormArgs a, int warp_teams, int stages) {
+  __shared__ __align__(16) float buf[2][32];
+  if (threadIdx.x < 64) buf[threadIdx.x >> 5][threadIdx.x & 31] = 0.f;
+  extern __shared__ __align__(128) unsigned char smem[];
   griddep_wait();
   const int nw = blockDim.x >> 5;
   const int team = warp_teams ? 32 : blockDim.x;
@@ -106,70 +233,105 @@ __global__ void __launch_bounds__(512) norm_fwd_kernel(const __grid_constant__ N
   const i64 c0 = (i64)grp * a.gs;
   const i64 slot = warp_teams ? (i64)blockIdx.x * nw + (threadIdx.x >> 5) : blockIdx.x;
   const i64 step = warp_teams ? (i64)gridDim.x * nw : gridDim.x;
-  float w[K][V], b[K][V];
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const int c = col_of<V>(k, team, t) + j;
-      w[k][j] = c < a.gs ? param<T>(a.w, c0 + c, a.w_f32) : 0.f;
-      b[k][j] = c < a.gs && a.b ? param<T>(a.b, c0 + c, a.w_f32) : 0.f;
-    }
+  constexpr int kArrays = GATE ? 2 : 1;
+  Ring ring;
+  auto fill = [&](i64 row, unsigned s) {
+    if (row >= a.rows) return;
+    const void* src[kArrays];
+    src[0] = static_cast<const T*>(a.x) + row * a.xs + c0;
+    if (GATE) src[kArrays - 1] = static_cast<const T*>(a.z) + row * a.zs + c0;
+    ring_fill<kArrays>(ring, s, src);
+  };
+  const unsigned char *sw = nullptr, *sb = nullptr;
+  if (RING) {
+    unsigned char* to = smem + 128 + stages * (unsigned)(a.gs * sizeof(T) * kArrays);
+    sw = to;
+    sb = stage_params<T>(a, c0, to);
+    ring = ring_make(smem, stages, a.gs * sizeof(T), kArrays);
+    if (threadIdx.x == 0)
+      for (int n = 0; n < stages; ++n) fill(slot + n * step, n);
   }
+  __syncthreads();
   int ph = 0;
+  RingAt at;
   for (i64 row = slot; row < a.rows; row += step) {
-    float u[K][V], s[GATE ? K : 1][V];
-    float sum = 0.f;
+    // Values in pairs (packed fp32 math); a thread has an even number of them.
+    constexpr int N = K * V;
+    float uf[K][V], sf[GATE ? K : 1][V];
+    if (RING) (void)mbar_wait(&ring.full[at.s], at.phase);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int c = col_of<V>(k, team, t);
-      load_cols<T, V>(a.x, row * a.xs + c0 + c, c < a.gs, u[k]);
-      if (GATE) load_cols<T, V>(a.z, row * a.zs + c0 + c, c < a.gs, s[k]);
+      if (RING) {
+        const unsigned char* st = ring.base + at.s * ring.stage;
+        smem_cols<T, V>(st, c, c < a.gs, uf[k]);
+        if (GATE) smem_cols<T, V>(st + ring.bytes, c, c < a.gs, sf[k]);
+      } else {
+        load_cols<T, V>(a.x, row * a.xs + c0 + c, c < a.gs, uf[k]);
+        if (GATE) load_cols<T, V>(a.z, row * a.zs + c0 + c, c < a.gs, sf[k]);
+      }
     }
+    float2 u[N / 2], s[GATE ? N / 2 : 1];
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        if (GATE) {
-          s[k][j] = silu_f(s[k][j]);
-          if (a.gate_first) u[k][j] *= s[k][j];
-        }
-        sum += u[k][j];
+    for (int i = 0; i < N / 2; ++i) {
+      u[i] = f2(uf[2 * i / V][2 * i % V], uf[(2 * i + 1) / V][(2 * i + 1) % V]);
+      if (GATE) {
+        s[i] = silu2(f2(sf[2 * i / V][2 * i % V], sf[(2 * i + 1) / V][(2 * i + 1) % V]));
+        if (a.gate_first) u[i] = mul2(u[i], s[i]);
       }
     }
     float mu = 0.f;
     if (a.layer) {
-      mu = team_sum(f2(sum, 0.f), !warp_teams, buf[ph], nw).x * a.inv;
+      float2 sum = f2(0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i) sum = add2(sum, u[i]);
+      mu = team_sum(sum.x + sum.y, !warp_teams, buf[ph], nw) * a.inv;
       ph ^= 1;
-    }
-    float sq = 0.f;
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      if (col_of<V>(k, team, t) < a.gs) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-          u[k][j] -= mu;
-          sq = fmaf(u[k][j], u[k][j], sq);
-        }
+      for (int i = 0; i < N / 2; ++i) {
+        // Columns past the group's end stay 0.
+        u[i].x = col_of<V>(2 * i / V, team, t) < a.gs ? u[i].x - mu : 0.f;
+        u[i].y = col_of<V>((2 * i + 1) / V, team, t) < a.gs ? u[i].y - mu : 0.f;
       }
     }
-    const float var = team_sum(f2(sq, 0.f), !warp_teams, buf[ph], nw).x * a.inv;
+    float2 sq = f2(0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) sq = fma2(u[i], u[i], sq);
+    const float var = team_sum(sq.x + sq.y, !warp_teams, buf[ph], nw) * a.inv;
     ph ^= 1;
+    if (RING) {
+      if (threadIdx.x == 0) fill(row + ring.stages * step, at.s);
+      at.next(ring.stages);
+    }
     const float r = 1.f / sqrtf(var + a.eps);
     if (t == 0) {
       if (a.rstd) a.rstd[row * a.groups + grp] = r;
       if (a.mean) a.mean[row * a.groups + grp] = mu;
     }
 #pragma unroll
+    for (int i = 0; i < N / 2; ++i) u[i] = mul2(u[i], f2(r, r));
+#pragma unroll
     for (int k = 0; k < K; ++k) {
       const int c = col_of<V>(k, team, t);
       if (c < a.gs) {
+        float w[V], b[V], o[V];
+        if constexpr (RING) {
+          smem_params<T, V>(sw, c, a.w_f32, w);
+          if (a.b) smem_params<T, V>(sb, c, a.w_f32, b);
+        } else {
+          load_params<T, V>(a.w, c0 + c, a.w_f32, w);
+          if (a.b) load_params<T, V>(a.b, c0 + c, a.w_f32, b);
+        }
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          u[k][j] = fmaf(u[k][j] * r, w[k][j], b[k][j]);
-          if (GATE && !a.gate_first) u[k][j] *= s[k][j];
+          const float2 u2 = u[(k * V + j) / 2];
+          o[j] = fmaf((k * V + j) % 2 ? u2.y : u2.x, w[j], a.b ? b[j] : 0.f);
+          if (GATE && !a.gate_first) {
+            const float2 s2 = s[(k * V + j) / 2];
+            o[j] *= (k * V + j) % 2 ? s2.y : s2.x;
+          }
         }
-        store_cols<T, V>(a.y, row * a.ys + c0 + c, u[k]);
+        store_cols<T, V>(a.y, row * a.ys + c0 + c, o);
       }
     }
   }
@@ -177,7 +339,7 @@ __global__ void __launch_bounds__(512) norm_fwd_kernel(const __grid_constant__ N
 
 // ---- backward ----
 template <typename T, int V, int K, bool GATE>
-__global__ void __launch_bounds__(512) norm_bwd_kernel(const __grid_constant__ NormArgs a, int warp_teams) {
+__global__ void __launch_bounds__(512) norm_bwd_kernel(const __grid_constant__ NormArgs a, int warp_teams, int) {
   __shared__ float2 buf[2][32];
   griddep_wait();
   const int nw = blockDim.x >> 5;
@@ -187,20 +349,19 @@ __global__ void __launch_bounds__(512) norm_bwd_kernel(const __grid_constant__ N
   const i64 c0 = (i64)grp * a.gs;
   const i64 slot = warp_teams ? (i64)blockIdx.x * nw + (threadIdx.x >> 5) : blockIdx.x;
   const i64 step = warp_teams ? (i64)gridDim.x * nw : gridDim.x;
-  float w[K][V], dw[K][V], db[K][V];
+  float dw[K][V], db[K][V];
 #pragma unroll
   for (int k = 0; k < K; ++k) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const int c = col_of<V>(k, team, t) + j;
-      w[k][j] = c < a.gs ? param<T>(a.w, c0 + c, a.w_f32) : 0.f;
-      dw[k][j] = db[k][j] = 0.f;
-    }
+    for (int j = 0; j < V; ++j) dw[k][j] = db[k][j] = 0.f;
   }
   int ph = 0;
   for (i64 row = slot; row < a.rows; row += step) {
-    // h: the normalised values; g: dO * w; both in registers for the sums.
+    // h: the normalised values (gate first: x); g: dO * w; both in registers
+    // for the second pass.
     float h[K][V], g[K][V], z[GATE ? K : 1][V];
+    const float r = a.rstd[row * a.groups + grp];
+    const float mu = a.layer ? a.mean[row * a.groups + grp] : 0.f;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int c = col_of<V>(k, team, t);
@@ -208,14 +369,14 @@ __global__ void __launch_bounds__(512) norm_bwd_kernel(const __grid_constant__ N
       load_cols<T, V>(a.dy, row * a.dys + c0 + c, c < a.gs, g[k]);
       if (GATE) load_cols<T, V>(a.z, row * a.zs + c0 + c, c < a.gs, z[k]);
     }
-    const float r = a.rstd[row * a.groups + grp];
-    const float mu = a.layer ? a.mean[row * a.groups + grp] : 0.f;
     float c1 = 0.f, c2 = 0.f;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int c = col_of<V>(k, team, t);
       if (c < a.gs) {
-        float dz[V];
+        float w[V], b[V], dz[V];
+        load_params<T, V>(a.w, c0 + c, a.w_f32, w);
+        if (GATE && !a.gate_first && a.b) load_params<T, V>(a.b, c0 + c, a.w_f32, b);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
           float u = h[k][j], d = g[k][j];
@@ -227,17 +388,16 @@ __global__ void __launch_bounds__(512) norm_bwd_kernel(const __grid_constant__ N
           if (GATE && a.gate_first) u *= si;
           const float hh = (u - mu) * r;
           if (GATE && !a.gate_first) {
-            const float o = fmaf(hh, w[k][j], a.b ? param<T>(a.b, c0 + c + j, a.w_f32) : 0.f);
+            const float o = fmaf(hh, w[j], a.b ? b[j] : 0.f);
             dz[j] = d * o * (sg * fmaf(z[k][j], 1.f - sg, 1.f));
             d *= si;
           }
           dw[k][j] = fmaf(d, hh, dw[k][j]);
-          db[k][j] += d;
-          const float gg = d * w[k][j];
+          if (a.b) db[k][j] += d;
+          const float gg = d * w[j];
           c1 = fmaf(gg, hh, c1);
           c2 += gg;
           g[k][j] = gg;
-          // Gate first: x is needed again and h follows from it; else h is.
           if (!(GATE && a.gate_first)) h[k][j] = hh;
         }
         if (GATE && !a.gate_first) store_cols<T, V>(a.dz, row * a.dzs + c0 + c, dz);
@@ -268,7 +428,6 @@ __global__ void __launch_bounds__(512) norm_bwd_kernel(const __grid_constant__ N
       }
     }
   }
-  if (slot >= a.slots) return;
 #pragma unroll
   for (int k = 0; k < K; ++k) {
 #pragma unroll
@@ -277,6 +436,137 @@ __global__ void __launch_bounds__(512) norm_bwd_kernel(const __grid_constant__ N
       if (c < a.gs) {
         a.part[slot * a.dim + c0 + c] = dw[k][j];
         if (a.b) a.part[((i64)a.slots + slot) * a.dim + c0 + c] = db[k][j];
+      }
+    }
+  }
+}
+
+// The same with rows in the ring: the second pass reads them from there once
+// more, so that only the sums over rows stay in registers and three blocks of
+// 320 threads share an SM.  A row's stage is filled again at the next row's
+// barrier.
+template <typename T, int V, int K, bool GATE>
+__global__ void __launch_bounds__(512, 2) norm_bwd_ring_kernel(const __grid_constant__ NormArgs a, int, int stages) {
+  __shared__ float2 buf[2][32];
+  __shared__ __align__(16) float buf1[2][32];
+  if (threadIdx.x < 64) buf1[threadIdx.x >> 5][threadIdx.x & 31] = 0.f;
+  extern __shared__ __align__(128) unsigned char smem[];
+  griddep_wait();
+  const int nw = blockDim.x >> 5, team = blockDim.x, t = threadIdx.x;
+  const int grp = blockIdx.y;
+  const i64 c0 = (i64)grp * a.gs;
+  constexpr int kArrays = GATE ? 3 : 2;
+  unsigned char* sw = smem + 128 + stages * (unsigned)(a.gs * sizeof(T) * kArrays);
+  const unsigned char* sb = stage_params<T>(a, c0, sw);
+  const Ring ring = ring_make(smem, stages, a.gs * sizeof(T), kArrays);
+  auto fill = [&](i64 row, unsigned s) {
+    if (row >= a.rows) return;
+    const void* src[kArrays];
+    src[0] = static_cast<const T*>(a.x) + row * a.xs + c0;
+    src[1] = static_cast<const T*>(a.dy) + row * a.dys + c0;
+    if (GATE) src[kArrays - 1] = static_cast<const T*>(a.z) + row * a.zs + c0;
+    ring_fill<kArrays>(ring, s, src);
+  };
+  if (t == 0)
+    for (int n = 0; n < stages; ++n) fill(blockIdx.x + (i64)n * gridDim.x, n);
+  __syncthreads();
+  float2 dw[K][V / 2], db[K][V / 2];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+#pragma unroll
+    for (int j = 0; j < V / 2; ++j) dw[k][j] = db[k][j] = f2(0.f, 0.f);
+  }
+  unsigned n = 0, last = 0;
+  RingAt at;
+  for (i64 row = blockIdx.x; row < a.rows; row += gridDim.x, ++n) {
+    const float r = a.rstd[row * a.groups + grp];
+    const float mu = a.layer ? a.mean[row * a.groups + grp] : 0.f;
+    (void)mbar_wait(&ring.full[at.s], at.phase);
+    const unsigned char* st = ring.base + at.s * ring.stage;
+    float2 c1 = f2(0.f, 0.f), c2 = f2(0.f, 0.f);
+    const float2 rr = f2(r, r), nmu = f2(-mu, -mu);
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int c = col_of<V>(k, team, t);
+      if (c < a.gs) {
+        float xf[V], df[V], zf[V], wf[V];
+        smem_cols<T, V>(st, c, true, xf);
+        smem_cols<T, V>(st + ring.bytes, c, true, df);
+        if (GATE) smem_cols<T, V>(st + 2 * ring.bytes, c, true, zf);
+        smem_params<T, V>(sw, c, a.w_f32, wf);
+#pragma unroll
+        for (int j = 0; j < V / 2; ++j) {
+          float2 x = f2(xf[2 * j], xf[2 * j + 1]), d = f2(df[2 * j], df[2 * j + 1]);
+          if (GATE) {
+            const float2 si = silu2(f2(zf[2 * j], zf[2 * j + 1]));
+            if (a.gate_first)
+              x = mul2(x, si);
+            else
+              d = mul2(d, si);
+          }
+          const float2 hh = mul2(add2(x, nmu), rr);
+          dw[k][j] = fma2(d, hh, dw[k][j]);
+          if (a.b) db[k][j] = add2(db[k][j], d);
+          const float2 g = mul2(d, f2(wf[2 * j], wf[2 * j + 1]));
+          c1 = fma2(g, hh, c1);
+          if (a.layer) c2 = add2(c2, g);
+        }
+      }
+    }
+    const float2 m = a.layer ? team_sum(f2(c1.x + c1.y, c2.x + c2.y), true, buf[n & 1], nw)
+                             : f2(team_sum(c1.x + c1.y, true, buf1[n & 1], nw), 0.f);
+    if (t == 0 && n > 0) fill(row + (i64)(ring.stages - 1) * gridDim.x, last);
+    last = at.s;
+    at.next(ring.stages);
+    const float2 m1 = f2(m.x * a.inv, m.x * a.inv), m2 = f2(m.y * a.inv, m.y * a.inv);
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int c = col_of<V>(k, team, t);
+      if (c < a.gs) {
+        float xf[V], df[V], zf[V], wf[V], bf[V];
+        smem_cols<T, V>(st, c, true, xf);
+        smem_cols<T, V>(st + ring.bytes, c, true, df);
+        if (GATE) smem_cols<T, V>(st + 2 * ring.bytes, c, true, zf);
+        smem_params<T, V>(sw, c, a.w_f32, wf);
+        if (GATE && !a.gate_first && a.b) smem_params<T, V>(sb, c, a.w_f32, bf);
+#pragma unroll
+        for (int j = 0; j < V / 2; ++j) {
+          const float2 x = f2(xf[2 * j], xf[2 * j + 1]), d = f2(df[2 * j], df[2 * j + 1]), w = f2(wf[2 * j], wf[2 * j + 1]);
+          float2 dx;
+          if (GATE) {
+            const float2 z = f2(zf[2 * j], zf[2 * j + 1]), one = f2(1.f, 1.f);
+            const float2 sg = sigmoid2(z), si = mul2(z, sg), gr = mul2(sg, fma2(z, fma2(sg, f2(-1.f, -1.f), one), one));
+            float2 dz;
+            if (a.gate_first) {
+              const float2 hh = mul2(add2(mul2(x, si), nmu), rr), tt = fma2(hh, m1, m2);
+              const float2 du = mul2(rr, fma2(d, w, f2(-tt.x, -tt.y)));
+              dz = mul2(mul2(du, x), gr);
+              dx = mul2(du, si);
+            } else {
+              const float2 hh = mul2(add2(x, nmu), rr), tt = fma2(hh, m1, m2);
+              dz = mul2(mul2(d, fma2(hh, w, a.b ? f2(bf[2 * j], bf[2 * j + 1]) : f2(0.f, 0.f))), gr);
+              dx = mul2(rr, fma2(mul2(d, si), w, f2(-tt.x, -tt.y)));
+            }
+            zf[2 * j] = dz.x, zf[2 * j + 1] = dz.y;
+          } else {
+            const float2 tt = fma2(mul2(add2(x, nmu), rr), m1, m2);
+            dx = mul2(rr, fma2(d, w, f2(-tt.x, -tt.y)));
+          }
+          xf[2 * j] = dx.x, xf[2 * j + 1] = dx.y;
+        }
+        store_cols<T, V>(a.dx, row * a.dxs + c0 + c, xf);
+        if (GATE) store_cols<T, V>(a.dz, row * a.dzs + c0 + c, zf);
+      }
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const int c = col_of<V>(k, team, t) + j;
+      if (c < a.gs) {
+        a.part[(i64)blockIdx.x * a.dim + c0 + c] = j % 2 ? dw[k][j / 2].y : dw[k][j / 2].x;
+        if (a.b) a.part[((i64)a.slots + blockIdx.x) * a.dim + c0 + c] = j % 2 ? db[k][j / 2].y : db[k][j / 2].x;
       }
     }
   }
@@ -402,8 +692,10 @@ __global__ void __launch_bounds__(512) norm_wide_bwd_kernel(const __grid_constan
 
 struct NormPlan {
   int v, k;          // columns per access, accesses per thread; k == 0: the wide kernels
+  int stages;        // ring of rows; 0: none
   int threads, warp_teams;
   i64 blocks;        // per group
+  unsigned smem;
   int slots;
 };
 
@@ -411,7 +703,7 @@ bool aligned(const void* p, i64 pitch, int esize) {
   return p == nullptr || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && (pitch * esize) % 16 == 0);
 }
 
-constexpr int kMaxTeam = 512;  // threads: 128 registers each at one block per SM
+constexpr int kMaxTeam = 512;
 
 int plan_norm(const char* what, const cc1d_gated_norm_params* p, bool bwd, NormArgs* a, NormPlan* plan, bool* empty) {
   if (p == nullptr) return report_error(CC1D_ERR_INVALID_ARGUMENT, "%s: params is NULL", what);
@@ -437,22 +729,24 @@ int plan_norm(const char* what, const cc1d_gated_norm_params* p, bool bwd, NormA
                 0, p->eps, 1.f / (float)p->group_size, p->layer ? 1 : 0, p->gate_first ? 1 : 0,
                 p->weight_dtype == CC1D_F32 ? 1 : 0};
   const int es = p->dtype == CC1D_F32 ? 4 : 2, wide = 16 / es;
-  bool vec = a->gs % wide == 0 && aligned(p->x, p->x_row_stride, es) && aligned(p->z, p->z_row_stride, es);
+  bool vec = a->gs % wide == 0 && aligned(p->weight, 0, es) && aligned(p->bias, 0, es) && aligned(p->x, p->x_row_stride, es) && aligned(p->z, p->z_row_stride, es);
   vec = vec && (bwd ? aligned(p->dy, p->dy_row_stride, es) && aligned(p->dx, p->dx_row_stride, es) &&
                           aligned(p->dz, p->dz_row_stride, es)
                     : aligned(p->y, p->y_row_stride, es));
   plan->v = vec ? wide : 1;
   const i64 acc = ceil_div(a->gs, plan->v);  // accesses per row and array
-  // Values per thread: up to 32 forward, 16 backward (it holds three arrays
-  // and the two sums); the team grows with the group.
-  const int most = std::max(1, (bwd ? 16 : 32) / plan->v);
-  plan->k = 1;
-  while (plan->k < std::min(most, 8) && acc > 32 * plan->k) plan->k *= 2;
+  // Values per thread: one vector (or four single ones) at first, up to 16
+  // values where a warp can then hold the group, or where the team would pass
+  // 512 threads.
+  const int most = 16 / plan->v;
+  plan->k = plan->v == 1 ? 4 : 1;
+  while (plan->k < most && (acc > 512 * plan->k || (acc > 32 * plan->k && acc <= 64 * plan->k))) plan->k *= 2;
   const i64 team = ceil_div(acc, plan->k);
   DeviceInfo dev;
   const cudaError_t e = device_info(&dev);
   const int sms = e == cudaSuccess ? dev.sms : 148;
   if (e != cudaSuccess) (void)cudaGetLastError();  // sizes may be asked for without a GPU
+  plan->stages = 0;
   if (team > kMaxTeam) {
     plan->k = 0;
     plan->threads = 512;
@@ -463,10 +757,22 @@ int plan_norm(const char* what, const cc1d_gated_norm_params* p, bool bwd, NormA
     plan->warp_teams = team <= 32;
     plan->threads = plan->warp_teams ? 128 : (int)ceil_div(team, 32) * 32;
     const int per_block = plan->warp_teams ? 4 : 1;
-    // Teams walk rows: enough blocks to fill the SMs' threads once.
-    const i64 fill = ceil_div((i64)sms * std::max(1, (bwd ? 1024 : 2048) / plan->threads), a->groups);
+    // Teams walk rows: blocks for as many threads as the registers hold.
+    const int resident = std::max(1, 1024 / plan->threads);
+    const unsigned stage = (unsigned)(a->gs * es) * ((bwd ? 2 : 1) + (p->z ? 1 : 0));
+    if (!plan->warp_teams && vec) {
+      // A ring when rows per block are many, of 2 to 4 stages in what shared
+      // memory the resident blocks have.
+      const i64 fill = ceil_div((i64)sms * resident, a->groups);
+      const int room = 220 * 1024 / resident;
+      const int params = a->gs * (a->w_f32 ? 4 : es) * (p->bias ? 2 : 1);
+      const int stages = std::min(4, (int)((room - 1024 - params) / (int)stage));
+      if (stages >= 2 && p->rows >= 4 * fill) plan->stages = stages;
+    }
+    const i64 fill = ceil_div((i64)sms * resident, a->groups);
     plan->blocks = std::max<i64>(1, std::min<i64>(ceil_div(p->rows, per_block), fill));
     plan->slots = (int)(plan->blocks * per_block);
+    plan->smem = plan->stages ? 128 + plan->stages * stage + a->gs * (a->w_f32 ? 4 : es) * (p->bias ? 2 : 1) : 0;
   }
   a->slots = plan->slots;
   return CC1D_OK;
@@ -476,27 +782,59 @@ size_t norm_workspace(const NormArgs& a, const NormPlan& plan) {
   return (size_t)plan.slots * a.dim * sizeof(float) * (a.b ? 2 : 1);
 }
 
-template <typename T, int V, int K>
+template <typename KERNEL>
+cudaError_t launch_team(KERNEL kernel, std::atomic<uint64_t>& attr_done, const NormArgs& a, const NormPlan& pl, cudaStream_t s) {
+  if (pl.smem > 48 * 1024) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = dev >= 0 && dev < 64 ? (1ull << dev) : 0ull;
+    if (bit == 0 || !(attr_done.load(std::memory_order_acquire) & bit)) {
+      e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 222 * 1024);
+      if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+      if (e != cudaSuccess) return e;
+      attr_done.fetch_or(bit, std::memory_order_acq_rel);
+    }
+  }
+  return launch_pdl(kernel, dim3((unsigned)pl.blocks, (unsigned)a.groups), dim3(pl.threads), pl.smem, s, a, pl.warp_teams,
+                    pl.stages);
+}
+
+template <typename T, int V, int K, bool GATE, bool RING>
 cudaError_t launch_norm_k(const NormArgs& a, const NormPlan& pl, bool bwd, cudaStream_t s) {
-  const dim3 grid((unsigned)pl.blocks, (unsigned)a.groups), block(pl.threads);
-  if (bwd)
-    return a.z ? launch_pdl(norm_bwd_kernel<T, V, K, true>, grid, block, 0, s, a, pl.warp_teams)
-               : launch_pdl(norm_bwd_kernel<T, V, K, false>, grid, block, 0, s, a, pl.warp_teams);
-  return a.z ? launch_pdl(norm_fwd_kernel<T, V, K, true>, grid, block, 0, s, a, pl.warp_teams)
-             : launch_pdl(norm_fwd_kernel<T, V, K, false>, grid, block, 0, s, a, pl.warp_teams);
+  static std::atomic<uint64_t> fwd_done{0}, bwd_done{0};
+  if (!bwd) return launch_team(norm_fwd_kernel<T, V, K, GATE, RING>, fwd_done, a, pl, s);
+  if constexpr (RING)
+    return launch_team(norm_bwd_ring_kernel<T, V, K, GATE>, bwd_done, a, pl, s);
+  else
+    return launch_team(norm_bwd_kernel<T, V, K, GATE>, bwd_done, a, pl, s);
+}
+
+template <typename T, int V, int K>
+cudaError_t launch_norm_g(const NormArgs& a, const NormPlan& pl, bool bwd, cudaStream_t s) {
+  if constexpr (V > 1) {
+    if (pl.stages) return a.z ? launch_norm_k<T, V, K, true, true>(a, pl, bwd, s) : launch_norm_k<T, V, K, false, true>(a, pl, bwd, s);
+  }
+  return a.z ? launch_norm_k<T, V, K, true, false>(a, pl, bwd, s) : launch_norm_k<T, V, K, false, false>(a, pl, bwd, s);
 }
 
 template <typename T, int V>
 cudaError_t launch_norm_v(const NormArgs& a, const NormPlan& pl, bool bwd, cudaStream_t s) {
-  switch (pl.k) {
-    case 1: return launch_norm_k<T, V, 1>(a, pl, bwd, s);
-    case 2: return launch_norm_k<T, V, 2>(a, pl, bwd, s);
-    case 4:
-      if constexpr (V <= 8) return launch_norm_k<T, V, 4>(a, pl, bwd, s);
-      break;
-    case 8:
-      if constexpr (V <= 4) return launch_norm_k<T, V, 8>(a, pl, bwd, s);
-      break;
+  if constexpr (V == 1) {
+    switch (pl.k) {
+      case 4: return launch_norm_g<T, V, 4>(a, pl, bwd, s);
+      case 8: return launch_norm_g<T, V, 8>(a, pl, bwd, s);
+      case 16: return launch_norm_g<T, V, 16>(a, pl, bwd, s);
+    }
+  } else {
+    switch (pl.k) {
+      case 1: return launch_norm_g<T, V, 1>(a, pl, bwd, s);
+      case 2: return launch_norm_g<T, V, 2>(a, pl, bwd, s);
+      case 4:
+        if constexpr (V <= 4) return launch_norm_g<T, V, 4>(a, pl, bwd, s);
+        break;
+    }
   }
   return cudaErrorInvalidValue;
 }
@@ -554,6 +892,8 @@ int norm_run(const char* what, const cc1d_gated_norm_params* p, bool bwd, void* 
 }
 
 }  // namespace
+
+cudaError_t read_norm_wait_timeouts(unsigned* count) { return tu_read_wait_timeouts(count); }
 
 }  // namespace cc1d
 
