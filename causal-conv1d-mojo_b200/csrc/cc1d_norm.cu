@@ -171,19 +171,43 @@ __device__ __forceinline__ unsigned char* stage_params(const NormArgs& a, i64 c0
   return to + a.gs * es;  // the bias
 }
 
+// V adjacent values at p (shared or global memory, 16-byte aligned) as V / 2
+// pairs, and back.
 template <typename T, int V>
-__device__ __forceinline__ void smem_params(const unsigned char* p, int c, int f32, float (&o)[V]) {
-  if (f32) {
+__device__ __forceinline__ void get_pairs(const void* p, float2 (&o)[V / 2]) {
+  const uint4 w = *static_cast<const uint4*>(p);
+  if constexpr (sizeof(T) == 4) {
+    o[0] = f2(__uint_as_float(w.x), __uint_as_float(w.y));
+    o[1] = f2(__uint_as_float(w.z), __uint_as_float(w.w));
+  } else {
+    o[0] = Pair<T>::unpack(w.x);
+    o[1] = Pair<T>::unpack(w.y);
+    o[2] = Pair<T>::unpack(w.z);
+    o[3] = Pair<T>::unpack(w.w);
+  }
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void put_pairs(void* p, const float2 (&v)[V / 2]) {
+  uint4 w;
+  if constexpr (sizeof(T) == 4) {
+    w = make_uint4(__float_as_uint(v[0].x), __float_as_uint(v[0].y), __float_as_uint(v[1].x), __float_as_uint(v[1].y));
+  } else {
+    w = make_uint4(Pair<T>::pack(v[0]), Pair<T>::pack(v[1]), Pair<T>::pack(v[2]), Pair<T>::pack(v[3]));
+  }
+  *static_cast<uint4*>(p) = w;
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void param_pairs(const unsigned char* p, int c, int f32, float2 (&o)[V / 2]) {
+  if (sizeof(T) == 4 || f32) {
 #pragma unroll
-    for (int j = 0; j < V; j += 4) {
-      const float4 v = *reinterpret_cast<const float4*>(p + (c + j) * 4);
-      o[j] = v.x, o[j + 1] = v.y, o[j + 2] = v.z, o[j + 3] = v.w;
+    for (int j = 0; j < V / 2; j += 2) {
+      const float4 v = *reinterpret_cast<const float4*>(p + (c + 2 * j) * 4);
+      o[j] = f2(v.x, v.y), o[j + 1] = f2(v.z, v.w);
     }
   } else {
-    Pack<T, V> pk;
-    pk.raw = *reinterpret_cast<const typename Pack<T, V>::Raw*>(p + c * sizeof(T));
-#pragma unroll
-    for (int j = 0; j < V; ++j) o[j] = Cvt<T>::f(pk.v[j]);
+    get_pairs<T, V>(p + c * sizeof(T), o);
   }
 }
 
@@ -204,28 +228,15 @@ __device__ __forceinline__ Ring ring_make(unsigned char* smem, int stages, unsig
   return r;
 }
 
-template <typename T, int V>
-__device__ __forceinline__ void smem_cols(const unsigned char* row, int c, bool ok, float (&o)[V]) {
-  Pack<T, V> pk;
-  if (ok) {
-    pk.raw = *reinterpret_cast<const typename Pack<T, V>::Raw*>(row + c * sizeof(T));
-#pragma unroll
-    for (int j = 0; j < V; ++j) o[j] = Cvt<T>::f(pk.v[j]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < V; ++j) o[j] = 0.f;
-  }
-}
-
 // ---- forward ----
 // Team: one warp (several per block) when a group fits 32 * K * V columns,
-// else the block.  RING: block teams only.
-template <typename T, int V, int K, bool GATE, bool RING>
-__global__ void __launch_bounds__(512, RING ? 2 : 1) norm_fwd_kernel(const __grid_constant__ NormArgs a, int warp_teams, int stages) {
+// else the block.
+template <typename T, int V, int K, bool GATE>
+__global__ void __launch_bounds__(512) norm_fwd_kernel(const __grid_constant__ NormArgs a, int warp_teams, int) {
   __shared__ __align__(16) float buf[2][32];
   if (threadIdx.x < 64) buf[threadIdx.x >> 5][threadIdx.x & 31] = 0.f;
-  extern __shared__ __align__(128) unsigned char smem[];
   griddep_wait();
+  __syncthreads();
   const int nw = blockDim.x >> 5;
   const int team = warp_teams ? 32 : blockDim.x;
   const int t = warp_teams ? (threadIdx.x & 31) : threadIdx.x;
@@ -233,8 +244,82 @@ __global__ void __launch_bounds__(512, RING ? 2 : 1) norm_fwd_kernel(const __gri
   const i64 c0 = (i64)grp * a.gs;
   const i64 slot = warp_teams ? (i64)blockIdx.x * nw + (threadIdx.x >> 5) : blockIdx.x;
   const i64 step = warp_teams ? (i64)gridDim.x * nw : gridDim.x;
+  int ph = 0;
+  for (i64 row = slot; row < a.rows; row += step) {
+    float u[K][V], s[GATE ? K : 1][V];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int c = col_of<V>(k, team, t);
+      load_cols<T, V>(a.x, row * a.xs + c0 + c, c < a.gs, u[k]);
+      if (GATE) load_cols<T, V>(a.z, row * a.zs + c0 + c, c < a.gs, s[k]);
+    }
+    float sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        if (GATE) {
+          s[k][j] = silu_f(s[k][j]);
+          if (a.gate_first) u[k][j] *= s[k][j];
+        }
+        sum += u[k][j];
+      }
+    }
+    float mu = 0.f;
+    if (a.layer) {
+      mu = team_sum(sum, !warp_teams, buf[ph], nw) * a.inv;
+      ph ^= 1;
+    }
+    float sq = 0.f;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      if (col_of<V>(k, team, t) < a.gs) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          u[k][j] -= mu;
+          sq = fmaf(u[k][j], u[k][j], sq);
+        }
+      }
+    }
+    const float var = team_sum(sq, !warp_teams, buf[ph], nw) * a.inv;
+    ph ^= 1;
+    const float r = 1.f / sqrtf(var + a.eps);
+    if (t == 0) {
+      if (a.rstd) a.rstd[row * a.groups + grp] = r;
+      if (a.mean) a.mean[row * a.groups + grp] = mu;
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int c = col_of<V>(k, team, t);
+      if (c < a.gs) {
+        float w[V], b[V];
+        load_params<T, V>(a.w, c0 + c, a.w_f32, w);
+        if (a.b) load_params<T, V>(a.b, c0 + c, a.w_f32, b);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          u[k][j] = fmaf(u[k][j] * r, w[j], a.b ? b[j] : 0.f);
+          if (GATE && !a.gate_first) u[k][j] *= s[k][j];
+        }
+        store_cols<T, V>(a.y, row * a.ys + c0 + c, u[k]);
+      }
+    }
+  }
+}
+
+// The same with rows in the ring, in pairs (packed fp32 math).
+template <typename T, int V, int K, bool GATE>
+__global__ void __launch_bounds__(512, 2) norm_fwd_ring_kernel(const __grid_constant__ NormArgs a, int, int stages) {
+  __shared__ __align__(16) float buf[2][32];
+  extern __shared__ __align__(128) unsigned char smem[];
+  if (threadIdx.x < 64) buf[threadIdx.x >> 5][threadIdx.x & 31] = 0.f;
+  griddep_wait();
+  const int nw = blockDim.x >> 5, team = blockDim.x, t = threadIdx.x;
+  const int grp = blockIdx.y;
+  const i64 c0 = (i64)grp * a.gs, step = gridDim.x;
   constexpr int kArrays = GATE ? 2 : 1;
-  Ring ring;
+  unsigned char* sw = smem + 128 + stages * (unsigned)(a.gs * sizeof(T) * kArrays);
+  const unsigned char* sb = stage_params<T>(a, c0, sw);
+  const Ring ring = ring_make(smem, stages, a.gs * sizeof(T), kArrays);
   auto fill = [&](i64 row, unsigned s) {
     if (row >= a.rows) return;
     const void* src[kArrays];
@@ -242,96 +327,79 @@ __global__ void __launch_bounds__(512, RING ? 2 : 1) norm_fwd_kernel(const __gri
     if (GATE) src[kArrays - 1] = static_cast<const T*>(a.z) + row * a.zs + c0;
     ring_fill<kArrays>(ring, s, src);
   };
-  const unsigned char *sw = nullptr, *sb = nullptr;
-  if (RING) {
-    unsigned char* to = smem + 128 + stages * (unsigned)(a.gs * sizeof(T) * kArrays);
-    sw = to;
-    sb = stage_params<T>(a, c0, to);
-    ring = ring_make(smem, stages, a.gs * sizeof(T), kArrays);
-    if (threadIdx.x == 0)
-      for (int n = 0; n < stages; ++n) fill(slot + n * step, n);
-  }
-  __syncthreads();
+  if (t == 0)
+    for (int n = 0; n < stages; ++n) fill(blockIdx.x + n * step, n);
   int ph = 0;
   RingAt at;
-  for (i64 row = slot; row < a.rows; row += step) {
-    // Values in pairs (packed fp32 math); a thread has an even number of them.
-    constexpr int N = K * V;
-    float uf[K][V], sf[GATE ? K : 1][V];
-    if (RING) (void)mbar_wait(&ring.full[at.s], at.phase);
+  for (i64 row = blockIdx.x; row < a.rows; row += step) {
+    (void)mbar_wait(&ring.full[at.s], at.phase);
+    const unsigned char* st = ring.base + at.s * ring.stage;
+    float2 u[K][V / 2], s[GATE ? K : 1][V / 2];
+    float2 sq = f2(0.f, 0.f);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const int c = col_of<V>(k, team, t);
-      if (RING) {
-        const unsigned char* st = ring.base + at.s * ring.stage;
-        smem_cols<T, V>(st, c, c < a.gs, uf[k]);
-        if (GATE) smem_cols<T, V>(st + ring.bytes, c, c < a.gs, sf[k]);
-      } else {
-        load_cols<T, V>(a.x, row * a.xs + c0 + c, c < a.gs, uf[k]);
-        if (GATE) load_cols<T, V>(a.z, row * a.zs + c0 + c, c < a.gs, sf[k]);
-      }
-    }
-    float2 u[N / 2], s[GATE ? N / 2 : 1];
+      if (c < a.gs) {
+        get_pairs<T, V>(st + c * sizeof(T), u[k]);
+        if (GATE) get_pairs<T, V>(st + ring.bytes + c * sizeof(T), s[k]);
 #pragma unroll
-    for (int i = 0; i < N / 2; ++i) {
-      u[i] = f2(uf[2 * i / V][2 * i % V], uf[(2 * i + 1) / V][(2 * i + 1) % V]);
-      if (GATE) {
-        s[i] = silu2(f2(sf[2 * i / V][2 * i % V], sf[(2 * i + 1) / V][(2 * i + 1) % V]));
-        if (a.gate_first) u[i] = mul2(u[i], s[i]);
+        for (int j = 0; j < V / 2; ++j) {
+          if (GATE) s[k][j] = silu2(s[k][j]);
+          if (GATE && a.gate_first) u[k][j] = mul2(u[k][j], s[k][j]);
+        }
       }
     }
     float mu = 0.f;
     if (a.layer) {
       float2 sum = f2(0.f, 0.f);
 #pragma unroll
-      for (int i = 0; i < N / 2; ++i) sum = add2(sum, u[i]);
-      mu = team_sum(sum.x + sum.y, !warp_teams, buf[ph], nw) * a.inv;
-      ph ^= 1;
+      for (int k = 0; k < K; ++k) {
+        if (col_of<V>(k, team, t) < a.gs) {
 #pragma unroll
-      for (int i = 0; i < N / 2; ++i) {
-        // Columns past the group's end stay 0.
-        u[i].x = col_of<V>(2 * i / V, team, t) < a.gs ? u[i].x - mu : 0.f;
-        u[i].y = col_of<V>((2 * i + 1) / V, team, t) < a.gs ? u[i].y - mu : 0.f;
+          for (int j = 0; j < V / 2; ++j) sum = add2(sum, u[k][j]);
+        }
+      }
+      mu = team_sum(sum.x + sum.y, true, buf[ph], nw) * a.inv;
+      ph ^= 1;
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      if (col_of<V>(k, team, t) < a.gs) {
+#pragma unroll
+        for (int j = 0; j < V / 2; ++j) {
+          if (a.layer) u[k][j] = add2(u[k][j], f2(-mu, -mu));
+          sq = fma2(u[k][j], u[k][j], sq);
+        }
       }
     }
-    float2 sq = f2(0.f, 0.f);
-#pragma unroll
-    for (int i = 0; i < N / 2; ++i) sq = fma2(u[i], u[i], sq);
-    const float var = team_sum(sq.x + sq.y, !warp_teams, buf[ph], nw) * a.inv;
+    const float var = team_sum(sq.x + sq.y, true, buf[ph], nw) * a.inv;
     ph ^= 1;
-    if (RING) {
-      if (threadIdx.x == 0) fill(row + ring.stages * step, at.s);
-      at.next(ring.stages);
-    }
+    if (t == 0) fill(row + ring.stages * step, at.s);
+    at.next(ring.stages);
     const float r = 1.f / sqrtf(var + a.eps);
     if (t == 0) {
       if (a.rstd) a.rstd[row * a.groups + grp] = r;
       if (a.mean) a.mean[row * a.groups + grp] = mu;
     }
 #pragma unroll
-    for (int i = 0; i < N / 2; ++i) u[i] = mul2(u[i], f2(r, r));
-#pragma unroll
     for (int k = 0; k < K; ++k) {
       const int c = col_of<V>(k, team, t);
       if (c < a.gs) {
-        float w[V], b[V], o[V];
-        if constexpr (RING) {
-          smem_params<T, V>(sw, c, a.w_f32, w);
-          if (a.b) smem_params<T, V>(sb, c, a.w_f32, b);
-        } else {
-          load_params<T, V>(a.w, c0 + c, a.w_f32, w);
-          if (a.b) load_params<T, V>(a.b, c0 + c, a.w_f32, b);
-        }
+        float2 w[V / 2];
+        param_pairs<T, V>(sw, c, a.w_f32, w);
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const float2 u2 = u[(k * V + j) / 2];
-          o[j] = fmaf((k * V + j) % 2 ? u2.y : u2.x, w[j], a.b ? b[j] : 0.f);
-          if (GATE && !a.gate_first) {
-            const float2 s2 = s[(k * V + j) / 2];
-            o[j] *= (k * V + j) % 2 ? s2.y : s2.x;
-          }
+        for (int j = 0; j < V / 2; ++j) u[k][j] = mul2(mul2(u[k][j], f2(r, r)), w[j]);
+        if (a.b) {
+          float2 b[V / 2];
+          param_pairs<T, V>(sb, c, a.w_f32, b);
+#pragma unroll
+          for (int j = 0; j < V / 2; ++j) u[k][j] = add2(u[k][j], b[j]);
         }
-        store_cols<T, V>(a.y, row * a.ys + c0 + c, o);
+        if (GATE && !a.gate_first) {
+#pragma unroll
+          for (int j = 0; j < V / 2; ++j) u[k][j] = mul2(u[k][j], s[k][j]);
+        }
+        put_pairs<T, V>(static_cast<T*>(a.y) + row * a.ys + c0 + c, u[k]);
       }
     }
   }
@@ -489,16 +557,16 @@ __global__ void __launch_bounds__(512, 2) norm_bwd_ring_kernel(const __grid_cons
     for (int k = 0; k < K; ++k) {
       const int c = col_of<V>(k, team, t);
       if (c < a.gs) {
-        float xf[V], df[V], zf[V], wf[V];
-        smem_cols<T, V>(st, c, true, xf);
-        smem_cols<T, V>(st + ring.bytes, c, true, df);
-        if (GATE) smem_cols<T, V>(st + 2 * ring.bytes, c, true, zf);
-        smem_params<T, V>(sw, c, a.w_f32, wf);
+        float2 xs[V / 2], ds[V / 2], zs[V / 2], ws[V / 2];
+        get_pairs<T, V>(st + c * sizeof(T), xs);
+        get_pairs<T, V>(st + ring.bytes + c * sizeof(T), ds);
+        if (GATE) get_pairs<T, V>(st + 2 * ring.bytes + c * sizeof(T), zs);
+        param_pairs<T, V>(sw, c, a.w_f32, ws);
 #pragma unroll
         for (int j = 0; j < V / 2; ++j) {
-          float2 x = f2(xf[2 * j], xf[2 * j + 1]), d = f2(df[2 * j], df[2 * j + 1]);
+          float2 x = xs[j], d = ds[j];
           if (GATE) {
-            const float2 si = silu2(f2(zf[2 * j], zf[2 * j + 1]));
+            const float2 si = silu2(zs[j]);
             if (a.gate_first)
               x = mul2(x, si);
             else
@@ -507,7 +575,7 @@ __global__ void __launch_bounds__(512, 2) norm_bwd_ring_kernel(const __grid_cons
           const float2 hh = mul2(add2(x, nmu), rr);
           dw[k][j] = fma2(d, hh, dw[k][j]);
           if (a.b) db[k][j] = add2(db[k][j], d);
-          const float2 g = mul2(d, f2(wf[2 * j], wf[2 * j + 1]));
+          const float2 g = mul2(d, ws[j]);
           c1 = fma2(g, hh, c1);
           if (a.layer) c2 = add2(c2, g);
         }
@@ -523,18 +591,18 @@ __global__ void __launch_bounds__(512, 2) norm_bwd_ring_kernel(const __grid_cons
     for (int k = 0; k < K; ++k) {
       const int c = col_of<V>(k, team, t);
       if (c < a.gs) {
-        float xf[V], df[V], zf[V], wf[V], bf[V];
-        smem_cols<T, V>(st, c, true, xf);
-        smem_cols<T, V>(st + ring.bytes, c, true, df);
-        if (GATE) smem_cols<T, V>(st + 2 * ring.bytes, c, true, zf);
-        smem_params<T, V>(sw, c, a.w_f32, wf);
-        if (GATE && !a.gate_first && a.b) smem_params<T, V>(sb, c, a.w_f32, bf);
+        float2 xs[V / 2], ds[V / 2], zs[V / 2], ws[V / 2], bs[V / 2];
+        get_pairs<T, V>(st + c * sizeof(T), xs);
+        get_pairs<T, V>(st + ring.bytes + c * sizeof(T), ds);
+        if (GATE) get_pairs<T, V>(st + 2 * ring.bytes + c * sizeof(T), zs);
+        param_pairs<T, V>(sw, c, a.w_f32, ws);
+        if (GATE && !a.gate_first && a.b) param_pairs<T, V>(sb, c, a.w_f32, bs);
 #pragma unroll
         for (int j = 0; j < V / 2; ++j) {
-          const float2 x = f2(xf[2 * j], xf[2 * j + 1]), d = f2(df[2 * j], df[2 * j + 1]), w = f2(wf[2 * j], wf[2 * j + 1]);
+          const float2 x = xs[j], d = ds[j], w = ws[j];
           float2 dx;
           if (GATE) {
-            const float2 z = f2(zf[2 * j], zf[2 * j + 1]), one = f2(1.f, 1.f);
+            const float2 z = zs[j], one = f2(1.f, 1.f);
             const float2 sg = sigmoid2(z), si = mul2(z, sg), gr = mul2(sg, fma2(z, fma2(sg, f2(-1.f, -1.f), one), one));
             float2 dz;
             if (a.gate_first) {
@@ -544,18 +612,18 @@ __global__ void __launch_bounds__(512, 2) norm_bwd_ring_kernel(const __grid_cons
               dx = mul2(du, si);
             } else {
               const float2 hh = mul2(add2(x, nmu), rr), tt = fma2(hh, m1, m2);
-              dz = mul2(mul2(d, fma2(hh, w, a.b ? f2(bf[2 * j], bf[2 * j + 1]) : f2(0.f, 0.f))), gr);
+              dz = mul2(mul2(d, fma2(hh, w, a.b ? bs[j] : f2(0.f, 0.f))), gr);
               dx = mul2(rr, fma2(mul2(d, si), w, f2(-tt.x, -tt.y)));
             }
-            zf[2 * j] = dz.x, zf[2 * j + 1] = dz.y;
+            zs[j] = dz;
           } else {
             const float2 tt = fma2(mul2(add2(x, nmu), rr), m1, m2);
             dx = mul2(rr, fma2(d, w, f2(-tt.x, -tt.y)));
           }
-          xf[2 * j] = dx.x, xf[2 * j + 1] = dx.y;
+          xs[j] = dx;
         }
-        store_cols<T, V>(a.dx, row * a.dxs + c0 + c, xf);
-        if (GATE) store_cols<T, V>(a.dz, row * a.dzs + c0 + c, zf);
+        put_pairs<T, V>(static_cast<T*>(a.dx) + row * a.dxs + c0 + c, xs);
+        if (GATE) put_pairs<T, V>(static_cast<T*>(a.dz) + row * a.dzs + c0 + c, zs);
       }
     }
   }
@@ -804,11 +872,13 @@ cudaError_t launch_team(KERNEL kernel, std::atomic<uint64_t>& attr_done, const N
 template <typename T, int V, int K, bool GATE, bool RING>
 cudaError_t launch_norm_k(const NormArgs& a, const NormPlan& pl, bool bwd, cudaStream_t s) {
   static std::atomic<uint64_t> fwd_done{0}, bwd_done{0};
-  if (!bwd) return launch_team(norm_fwd_kernel<T, V, K, GATE, RING>, fwd_done, a, pl, s);
-  if constexpr (RING)
-    return launch_team(norm_bwd_ring_kernel<T, V, K, GATE>, bwd_done, a, pl, s);
-  else
-    return launch_team(norm_bwd_kernel<T, V, K, GATE>, bwd_done, a, pl, s);
+  if constexpr (RING) {
+    return bwd ? launch_team(norm_bwd_ring_kernel<T, V, K, GATE>, bwd_done, a, pl, s)
+               : launch_team(norm_fwd_ring_kernel<T, V, K, GATE>, fwd_done, a, pl, s);
+  } else {
+    return bwd ? launch_team(norm_bwd_kernel<T, V, K, GATE>, bwd_done, a, pl, s)
+               : launch_team(norm_fwd_kernel<T, V, K, GATE>, fwd_done, a, pl, s);
+  }
 }
 
 template <typename T, int V, int K>

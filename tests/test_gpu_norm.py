@@ -125,6 +125,16 @@ def test_norm_many_rows_and_fp32_weight(rows):
     assert all(torch.equal(got[k], again[k]) for k in got)
 
 
+@pytest.mark.parametrize("dtype,rows,dim,group,wdtype", [(BF, 2500, 5120, 5120, None), (FP16, 1900, 2056, 2056, F32),
+                                                        (F32, 2000, 2048, 2048, None), (BF, 1801, 3200, 1600, None)])
+@pytest.mark.parametrize("kind,gate,gate_first,bias", [
+    ("rms", False, True, False), ("rms", True, True, False), ("layer", True, False, True), ("layer", False, True, True),
+])
+def test_norm_many_wide_rows(dtype, rows, dim, group, wdtype, kind, gate, gate_first, bias):
+    """Several rows per block, so that they come through shared memory; rows that do not divide evenly."""
+    _check(_inputs(rows, dim, dtype, gate, bias, wdtype=wdtype, seed=dim), group, kind, gate_first)
+
+
 def test_norm_large_mean():
     """A layer norm of values far from zero: the variance is that of the centred values."""
     _check(_inputs(9, 1024, F32, False, True, seed=1, mean=300.0), 1024, "layer", True)
