@@ -513,7 +513,7 @@ __global__ void __launch_bounds__(512) norm_bwd_kernel(const __grid_constant__ N
 // more, so that only the sums over rows stay in registers and three blocks of
 // 320 threads share an SM.  A row's stage is filled again at the next row's
 // barrier.
-template <typename T, int V, int K, bool GATE>
+template <typename T, int V, int K, bool GATE, bool BIAS>
 __global__ void __launch_bounds__(512, 2) norm_bwd_ring_kernel(const __grid_constant__ NormArgs a, int, int stages) {
   __shared__ float2 buf[2][32];
   __shared__ __align__(16) float buf1[2][32];
@@ -538,11 +538,11 @@ __global__ void __launch_bounds__(512, 2) norm_bwd_ring_kernel(const __grid_cons
   if (t == 0)
     for (int n = 0; n < stages; ++n) fill(blockIdx.x + (i64)n * gridDim.x, n);
   __syncthreads();
-  float2 dw[K][V / 2], db[K][V / 2];
+  float2 dw[K][V / 2], db[BIAS ? K : 1][V / 2];
 #pragma unroll
   for (int k = 0; k < K; ++k) {
 #pragma unroll
-    for (int j = 0; j < V / 2; ++j) dw[k][j] = db[k][j] = f2(0.f, 0.f);
+    for (int j = 0; j < V / 2; ++j) dw[k][j] = db[BIAS ? k : 0][j] = f2(0.f, 0.f);
   }
   unsigned n = 0, last = 0;
   RingAt at;
@@ -574,7 +574,7 @@ __global__ void __launch_bounds__(512, 2) norm_bwd_ring_kernel(const __grid_cons
           }
           const float2 hh = mul2(add2(x, nmu), rr);
           dw[k][j] = fma2(d, hh, dw[k][j]);
-          if (a.b) db[k][j] = add2(db[k][j], d);
+          if (BIAS) db[BIAS ? k : 0][j] = add2(db[BIAS ? k : 0][j], d);
           const float2 g = mul2(d, ws[j]);
           c1 = fma2(g, hh, c1);
           if (a.layer) c2 = add2(c2, g);
@@ -596,7 +596,7 @@ __global__ void __launch_bounds__(512, 2) norm_bwd_ring_kernel(const __grid_cons
         get_pairs<T, V>(st + ring.bytes + c * sizeof(T), ds);
         if (GATE) get_pairs<T, V>(st + 2 * ring.bytes + c * sizeof(T), zs);
         param_pairs<T, V>(sw, c, a.w_f32, ws);
-        if (GATE && !a.gate_first && a.b) param_pairs<T, V>(sb, c, a.w_f32, bs);
+        if (BIAS && GATE && !a.gate_first) param_pairs<T, V>(sb, c, a.w_f32, bs);
 #pragma unroll
         for (int j = 0; j < V / 2; ++j) {
           const float2 x = xs[j], d = ds[j], w = ws[j];
@@ -612,7 +612,7 @@ __global__ void __launch_bounds__(512, 2) norm_bwd_ring_kernel(const __grid_cons
               dx = mul2(du, si);
             } else {
               const float2 hh = mul2(add2(x, nmu), rr), tt = fma2(hh, m1, m2);
-              dz = mul2(mul2(d, fma2(hh, w, a.b ? bs[j] : f2(0.f, 0.f))), gr);
+              dz = mul2(mul2(d, fma2(hh, w, BIAS ? bs[j] : f2(0.f, 0.f))), gr);
               dx = mul2(rr, fma2(mul2(d, si), w, f2(-tt.x, -tt.y)));
             }
             zs[j] = dz;
@@ -634,7 +634,7 @@ __global__ void __launch_bounds__(512, 2) norm_bwd_ring_kernel(const __grid_cons
       const int c = col_of<V>(k, team, t) + j;
       if (c < a.gs) {
         a.part[(i64)blockIdx.x * a.dim + c0 + c] = j % 2 ? dw[k][j / 2].y : dw[k][j / 2].x;
-        if (a.b) a.part[((i64)a.slots + blockIdx.x) * a.dim + c0 + c] = j % 2 ? db[k][j / 2].y : db[k][j / 2].x;
+        if (BIAS) a.part[((i64)a.slots + blockIdx.x) * a.dim + c0 + c] = j % 2 ? db[BIAS ? k : 0][j / 2].y : db[BIAS ? k : 0][j / 2].x;
       }
     }
   }
@@ -871,10 +871,11 @@ cudaError_t launch_team(KERNEL kernel, std::atomic<uint64_t>& attr_done, const N
 
 template <typename T, int V, int K, bool GATE, bool RING>
 cudaError_t launch_norm_k(const NormArgs& a, const NormPlan& pl, bool bwd, cudaStream_t s) {
-  static std::atomic<uint64_t> fwd_done{0}, bwd_done{0};
+  static std::atomic<uint64_t> fwd_done{0}, bwd_done{0}, bwd_bias_done{0};
   if constexpr (RING) {
-    return bwd ? launch_team(norm_bwd_ring_kernel<T, V, K, GATE>, bwd_done, a, pl, s)
-               : launch_team(norm_fwd_ring_kernel<T, V, K, GATE>, fwd_done, a, pl, s);
+    if (!bwd) return launch_team(norm_fwd_ring_kernel<T, V, K, GATE>, fwd_done, a, pl, s);
+    return a.b ? launch_team(norm_bwd_ring_kernel<T, V, K, GATE, true>, bwd_bias_done, a, pl, s)
+               : launch_team(norm_bwd_ring_kernel<T, V, K, GATE, false>, bwd_done, a, pl, s);
   } else {
     return bwd ? launch_team(norm_bwd_kernel<T, V, K, GATE>, bwd_done, a, pl, s)
                : launch_team(norm_fwd_kernel<T, V, K, GATE>, fwd_done, a, pl, s);
