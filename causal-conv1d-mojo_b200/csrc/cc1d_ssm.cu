@@ -417,7 +417,7 @@ int plan_scan(const cc1d_scan_params* p, ScanArgs* a, ScanPlan* plan) {
                 p->y, p->y_batch_stride, p->y_seq_stride, p->y_head_stride,
                 p->final_states, p->final_seq_stride, p->final_head_stride,
                 nullptr, nullptr, p->seqlen, (int)p->nheads, (int)p->headdim, (int)p->dstate, (int)p->ngroups,
-                (int)(p->nheads / p->ngroups), (int)nseq, 0, 1, 0,
+                (int)(p->nheads / p->ngroups), (int)nseq, 0, 1, 0, 0,
                 p->dt_softplus ? 1 : 0, p->dt_dtype == CC1D_F32 ? 1 : 0,
                 p->init_dtype == CC1D_F32 ? 1 : 0};
   a->seg_len = std::max<i64>(1, p->seqlen);
@@ -428,12 +428,41 @@ int plan_scan(const cc1d_scan_params* p, ScanArgs* a, ScanPlan* plan) {
   // the walk over tokens is done sooner.
   const i64 mean = p->cu_seqlens ? ceil_div(p->seqlen, nseq) : p->seqlen;
   plan->tc = mean >= 16 && scan_tc_eligible(p->dtype, *a, p->batch);
-  // Sequences are split when their rows alone do not fill the SMs (one CTA
+  DeviceInfo dev;
+  const cudaError_t de = device_info(&dev);
+  const i64 sms = de == cudaSuccess ? dev.sms : 148;
+  if (de != cudaSuccess) (void)cudaGetLastError();  // sizes may be asked for without a GPU
+  if (plan->tc && p->cu_seqlens == nullptr) {
+    // One CTA an SM, so rows run in waves.  Rows may be cut into k segments, all
+    // of them or those that fill no wave; the first pass over segments (states
+    // only) takes about 0.65 of the second's time, a wave about one block more.
+    const i64 rows = nseq * scan_tc_pairs(*a), blocks = ceil_div(p->seqlen, kScanBlock);
+    a->whole = rows;
+    double best = (double)ceil_div(rows, sms) * (blocks + 1);
+    for (int all = 0; all < 2; ++all) {
+      const i64 cut = all ? rows : rows % sms;
+      for (i64 k = 2; cut > 0 && k <= std::min<i64>(blocks / 2, 64); ++k) {
+        const i64 len = ceil_div(blocks, k);
+        if (ceil_div(blocks, len) != k) continue;
+        const double cost = (double)((rows - cut) / sms) * (blocks + 1) + (double)ceil_div(cut * k, sms) * (len + 1) +
+                            (double)ceil_div(cut * (k - 1), sms) * (0.65 * len + 1);
+        if (cost < 0.95 * best) {
+          best = cost;
+          plan->split = true;
+          a->whole = rows - cut;
+          a->seg_len = len * kScanBlock;
+          a->segs = (int)k;
+        }
+      }
+    }
+    return CC1D_OK;
+  }
+  // The others are split when their rows alone do not fill the SMs (one CTA
   // each on the tensor cores, about four blocks of the walk), into segments of
   // two blocks or 64 tokens at least; packed ones as if they were one.
   const i64 rows = (p->cu_seqlens ? 1 : nseq) * (plan->tc ? scan_tc_pairs(*a) : a->H * ceil_div(a->P, 64));
   const i64 least = plan->tc ? 2 * kScanBlock : 64, unit = plan->tc ? kScanBlock : 16;
-  const i64 segs = std::min<i64>((plan->tc ? 148 : 592) / rows, p->seqlen / least);
+  const i64 segs = std::min<i64>((plan->tc ? sms : 4 * sms) / rows, p->seqlen / least);
   if (segs > 1) {
     const i64 len = ceil_div(ceil_div(p->seqlen, segs), unit) * unit;
     const i64 longest = p->cu_seqlens && p->max_seqlen == 0 ? p->seqlen : p->cu_seqlens ? p->max_seqlen : p->seqlen;
@@ -449,7 +478,7 @@ int plan_scan(const cc1d_scan_params* p, ScanArgs* a, ScanPlan* plan) {
 
 size_t scan_workspace(const ScanArgs& a, const ScanPlan& plan) {
   if (plan.empty || !plan.split) return 0;
-  return (size_t)(a.items * a.H) * ((size_t)a.P * a.N + 1) * sizeof(float);
+  return (size_t)(plan.tc ? scan_tc_parts(a) : a.items * a.H) * ((size_t)a.P * a.N + 1) * sizeof(float);
 }
 
 template <typename T>
@@ -484,7 +513,7 @@ extern "C" int cc1d_scan(const cc1d_scan_params* p, void* stream) {
   if (rc != CC1D_OK) return rc;
   if (need > 0) {
     a.part = static_cast<float*>(p->workspace);
-    a.decay = a.part + (size_t)(a.items * a.H) * a.P * a.N;
+    a.decay = a.part + (size_t)(plan.tc ? scan_tc_parts(a) : a.items * a.H) * a.P * a.N;
   }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e = cudaSuccess;

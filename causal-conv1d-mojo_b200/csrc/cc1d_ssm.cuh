@@ -28,14 +28,15 @@ struct ScanArgs {
   const void* init; i64 is_s, is_h;
   void* y; i64 ys_b, ys_t, ys_h;
   float* fin; i64 fs_s, fs_h;
-  float* part;         // [items][H][P][N]: a segment's state from zero
-  float* decay;        // [items][H]: log2 of its decay
+  float* part;         // [segments][heads][P][N]: a segment's state from zero
+  float* decay;        // [segments][heads]: log2 of its decay
   i64 L;               // tokens of a row
   int H, P, N, G, R;   // R = H / G heads per group
   int nseq;
   i64 seg_len;         // tokens per segment
   int segs;            // segments per sequence (without cu)
   i64 items;           // upper bound of the number of segments
+  i64 whole;           // tensor cores, without cu: (sequence, heads) rows that are not cut
   int softplus, dt_f32, init_f32;
 };
 
@@ -118,6 +119,7 @@ __device__ __forceinline__ float scan_step(const ScanArgs& a, i64 off, float bia
 // segment, its tokens per block and its launch (the partial states first when
 // `part` is set).
 constexpr int kScanBlock = 128;
+i64 scan_tc_parts(const ScanArgs& a);  // partial states of a split launch
 bool scan_tc_eligible(int dtype, const ScanArgs& a, i64 batch);
 int scan_tc_pairs(const ScanArgs& a);
 cudaError_t launch_scan_tc(int dtype, const ScanArgs& a, i64 batch, cudaStream_t stream);

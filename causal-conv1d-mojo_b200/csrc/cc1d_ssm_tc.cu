@@ -276,11 +276,35 @@ __global__ void __launch_bounds__(kThreads, 1) scan_tc_kernel(const __grid_const
   const ScanArgs& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  griddep_wait();
+  // With partial states to compute, that launch comes first and lets this one
+  // start at once: its own wait is behind it by then, so what rows that are not
+  // cut read is there, and only segments wait for the partial states.
+  if (PART || a.part == nullptr || a.cu != nullptr || blockIdx.x >= a.whole) griddep_wait();
+  if (PART) griddep_launch_dependents();
   ScanItem it;
-  const i64 item = blockIdx.x / p.npairs;
-  const int pair = blockIdx.x % p.npairs;
-  if (!scan_locate(a, item, &it)) return;
+  int pair;
+  i64 part0;  // slot of segment 0 of this row's partial states; segment r is r * part_step behind
+  int part_step;
+  if (a.cu == nullptr) {
+    // The first `whole` rows (sequence, heads) run uncut, the others in segments.
+    const i64 x = (i64)blockIdx.x + (PART ? a.whole : 0), y = x - a.whole;
+    const i64 row = y < 0 ? x : a.whole + y / a.segs;
+    it.seq = (int)(row / p.npairs);
+    pair = (int)(row - (i64)it.seq * p.npairs);
+    it.nsegs = y < 0 ? 1 : a.segs;
+    it.seg = y < 0 ? 0 : (int)(y % a.segs);
+    it.batch = it.seq;
+    it.t0 = it.seg * a.seg_len;
+    it.t1 = y < 0 ? a.L : min(a.L, it.t0 + a.seg_len);
+    part0 = y - it.seg;
+    part_step = 1;
+  } else {
+    const i64 item = blockIdx.x / p.npairs;
+    pair = blockIdx.x % p.npairs;
+    if (!scan_locate(a, item, &it)) return;
+    part0 = it.first * p.npairs + pair;
+    part_step = p.npairs;
+  }
   if (PART && it.seg + 1 >= it.nsegs) return;
   const int g = pair / p.ppg;
   const int h0 = g * a.R + (pair % p.ppg) * (WIDE ? 1 : 2);
@@ -738,7 +762,7 @@ __global__ void __launch_bounds__(kThreads, 1) scan_tc_kernel(const __grid_const
         }
 #pragma unroll 1
         for (int r = 0; r < it.seg; ++r) {  // the earlier segments, in order
-          const i64 slot = (it.first + r) * a.H + h;
+          const i64 slot = (part0 + (i64)r * part_step) * (WIDE ? 1 : 2) + hs;
           const float dc = ex2_approx(a.decay[slot]);
           const float* part = a.part + slot * a.P * a.N + e0;
 #pragma unroll
@@ -912,7 +936,7 @@ __global__ void __launch_bounds__(kThreads, 1) scan_tc_kernel(const __grid_const
     if (live) {
       const i64 h = h0 + hs;
       if (PART) {
-        const i64 slot = item * a.H + h;
+        const i64 slot = (part0 + (i64)it.seg * part_step) * (WIDE ? 1 : 2) + hs;
         out = a.part + slot * a.P * a.N;
         if (pr == 0 && hf == 0) a.decay[slot] = total;
       } else if (a.fin && it.seg + 1 == it.nsegs) {
@@ -982,7 +1006,8 @@ cudaError_t launch_one(const TcArgs& t, cudaStream_t s) {
     if (e != cudaSuccess) return e;
     attr_done.fetch_or(bit, std::memory_order_acq_rel);
   }
-  return launch_pdl(scan_tc_kernel<T, TERMS, PART, WIDE>, dim3((unsigned)(t.a.items * t.npairs)), dim3(kThreads), kSmem, s, t);
+  const i64 grid = t.a.cu ? t.a.items * t.npairs : (PART ? 0 : t.a.whole) + ((i64)t.a.nseq * t.npairs - t.a.whole) * t.a.segs;
+  return launch_pdl(scan_tc_kernel<T, TERMS, PART, WIDE>, dim3((unsigned)grid), dim3(kThreads), kSmem, s, t);
 }
 
 template <typename T, bool WIDE>
@@ -1008,6 +1033,11 @@ bool tile_ok(const void* base, i64 unit, i64 heads, i64 s_h, i64 tokens, i64 s_t
 }  // namespace
 
 int scan_tc_pairs(const ScanArgs& a) { return a.P > 64 ? a.H : a.G * (int)ceil_div(a.R, 2); }
+
+i64 scan_tc_parts(const ScanArgs& a) {
+  const i64 pairs = scan_tc_pairs(a);
+  return (a.cu ? a.items * pairs : (a.nseq * pairs - a.whole) * a.segs) * (a.P > 64 ? 1 : 2);
+}
 
 bool scan_tc_eligible(int dtype, const ScanArgs& a, i64 batch) {
   if (dtype == 2 || a.P < 8 || a.P > 128 || a.P % 8 || a.N < 8 || a.N > 128 || a.N % 8) return false;
