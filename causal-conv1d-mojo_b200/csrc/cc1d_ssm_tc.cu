@@ -44,7 +44,8 @@
 //   warp 2       issues dS: the chains of y and of the state meet only where
 //                one needs the other, and one issuer for both would make each
 //                wait for the other's barriers
-//   warps 4-11   tokens: thread = token row.  Steps and decays of the next block;  M from G, in place in TMEM (16
+//   warps 4-11   tokens: thread = token row.  Steps, decays and the first unit of
+//                (w X)^T of the next block;  M from G, in place in TMEM (16
 //                fp32 columns become 8 + 8 of pairs, one head each); scales inter by exp(c_i), so that intra accumulates
 //                onto it; y + D x over x in shared memory
 //   warps 12-19  state: thread = row p of S, half of n.  (w X)^T into TMEM,
@@ -55,8 +56,11 @@
 // What a role does between two waits is kept short: with few warps it runs at
 // the latency of its instructions.
 //
-// A barrier tells only the last two phases apart, so one that its waiter
-// might see two blocks late is kept per stage.
+// A barrier tells only two phases apart: a waiter has to know that the phase
+// before the one it waits for is over, and the one after must not end before
+// it has looked.  So a waiter waits for every phase of a barrier in turn, and
+// barriers are kept per stage, or per unit of a block, where the other side
+// could be a block ahead.
 //
 // Every mbarrier wait is bounded; after one that gave up no wait waits, the
 // roles run to their ends, outstanding copies and products are waited for
@@ -102,7 +106,7 @@ struct Bars {
   uint64_t emptyB[2], emptyC;
   uint64_t cumF[2];
   uint64_t gR, iR, pR, yR, yF;
-  uint64_t wR[2], wF[2];
+  uint64_t wR[4], wF[4];  // of the units of a block
   uint64_t dR, dF, sR, end, endS;
   uint64_t xF[2], yS[2];  // the state's warps have read x and the steps; y is in x's place
   uint64_t xSync, mSync;  // among the state warps
@@ -212,7 +216,9 @@ __device__ __forceinline__ void tma_tile(void* dst, const CUtensorMap* map, uint
 
 // Bounded wait by a warp (or one lane).  One that gives up sets the abort
 // flag, and with the flag set no wait waits: every role then runs to its end
-// on whatever is there, within its buffers, and the kernel is over.
+// on whatever is there, within its buffers, and the kernel is over.  (The
+// copies stop at once: a load's barrier must not be armed a second time
+// before it has completed.)
 __device__ __forceinline__ void wait_for(uint64_t* bar, unsigned parity, int* abort_flag) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t.reg .u32 n, f;\n\t"
@@ -245,6 +251,10 @@ __device__ __forceinline__ void warp_arrive(uint64_t* bar) {
       : "memory");
 }
 
+// fp16: w X is scaled per row of dS.
+template <typename T>
+constexpr bool kRowScale = std::is_same<T, __half>::value;
+
 // Takes the leading 16-bit term off two values.  bf16 terms of a split are
 // cut, not rounded: the upper halves of the words, eight bits each, so that
 // three of them are the 24 bits of the value.
@@ -263,6 +273,60 @@ __device__ __forceinline__ uint32_t take_term(float2& v) {
     return w;
   }
 }
+
+// w X in units of 32 tokens.  x comes transposed out of shared memory
+// (ldmatrix), as lane l's columns p = l / 4 (+ 8, 16, 24) and tokens
+// 2 (l % 4), + 1 of eight; the 16x128b stores put that into TMEM as rows p
+// and columns of token pairs.  Of a unit a warp does 32 rows and 16 tokens:
+// matrices of 8 tokens by 8 columns in the order (first 8 tokens, second 8) x
+// (8 columns, next 8).
+template <typename T, int TERMS>
+struct Units {
+  uint32_t row, col0, col1;
+  int token, hf;
+
+  __device__ __forceinline__ Units(unsigned char* sm, int q, int half, int lane) {
+    row = smem_u32(sm) + kOffX + (q >> 1) * kBox + (16 * half + ((lane >> 4) << 3) + (lane & 7)) * 128;
+    col0 = (((q & 1) * 4 + ((lane >> 3) & 1)) ^ (lane & 7)) << 4;
+    col1 = col0 ^ (2 << 4);
+    token = 16 * half + 2 * (lane & 3);  // this lane's first token of a unit
+    hf = half;
+  }
+  __device__ __forceinline__ void load(unsigned s, unsigned un, uint32_t (&x)[8]) const {
+    const uint32_t at = row + s * kTile + un * (32 * 128);
+    ldmatrix_t(at + col0, x[0], x[1], x[2], x[3]);
+    ldmatrix_t(at + col1, x[4], x[5], x[6], x[7]);
+  }
+  // Unit n (of block n / 4, whose x is in stage s): u x g x, in terms, where
+  // dS's products read it, when they have read unit n - 2 there.
+  __device__ __forceinline__ void make(Bars* bar, uint32_t tm, unsigned s, unsigned n, const float* u, float g,
+                                       const float (&scale)[4]) const {
+    const unsigned un = n & 3;
+    uint32_t x[8];
+    load(s, un, x);
+    const float2 w0 = mul2(*reinterpret_cast<const float2*>(u + token + 32 * un), f2(g, g));
+    const float2 w1 = mul2(*reinterpret_cast<const float2*>(u + token + 32 * un + 8), f2(g, g));
+    if (n >= 2) wait_for(&bar->wF[(n - 2) & 3], ((n - 2) >> 2) & 1, &bar->abort);
+    tc_after();
+    uint32_t o[TERMS][8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float2 v = mul2((i & 2) ? w1 : w0, Pair<T>::unpack(x[i]));
+      if (kRowScale<T>) v = mul2(v, f2(scale[2 * (i >> 2) + (i & 1)], scale[2 * (i >> 2) + (i & 1)]));
+#pragma unroll
+      for (int k = 0; k < TERMS; ++k) o[k][i] = take_term<T, (TERMS > 1)>(v);
+    }
+    const uint32_t at = tm + kColW + (n & 1) * (16 * TERMS) + 8 * hf;
+#pragma unroll
+    for (int k = 0; k < TERMS; ++k) {
+      tm_st_16x128(at + 16 * k, o[k][0], o[k][1], o[k][2], o[k][3]);
+      tm_st_16x128(at + 16 * k + (16u << 16), o[k][4], o[k][5], o[k][6], o[k][7]);
+    }
+    tm_st_wait();
+    tc_before();
+    warp_arrive(&bar->wR[un]);
+  }
+};
 
 // TERMS: 16-bit terms of w X.  PART: only the segment's state from zero.
 // WIDE: one head of up to 128 columns instead of two of up to 64.
@@ -327,7 +391,7 @@ __global__ void __launch_bounds__(kThreads, 1) scan_tc_kernel(const __grid_const
     mbar_init(&bar->pR, 8);
     mbar_init(&bar->yR, 1);
     mbar_init(&bar->yF, 8);
-    for (int s = 0; s < 2; ++s) {
+    for (int s = 0; s < 4; ++s) {
       mbar_init(&bar->wR[s], 8);
       mbar_init(&bar->wF[s], 1);
     }
@@ -346,6 +410,10 @@ __global__ void __launch_bounds__(kThreads, 1) scan_tc_kernel(const __grid_const
   __syncthreads();
   tc_after();
   const uint32_t tmem = bar->tmem;
+  // The first unit of a block's w X is the tokens' warps' work, which else
+  // wait more than the state's.  (fp16: the row scale is of the whole block
+  // and would have to come first, so the state's warps do all.)
+  constexpr bool kShare = !kRowScale<T>;
   auto wait = [&](uint64_t& b, unsigned phase) { wait_for(&b, phase & 1, &bar->abort); };
 
   // Registers: 96 a thread at launch (61440 in all); the other warps take over
@@ -377,28 +445,36 @@ __global__ void __launch_bounds__(kThreads, 1) scan_tc_kernel(const __grid_const
         asm volatile("cp.async.bulk.commit_group;\n\tcp.async.bulk.wait_group.read 0;" ::: "memory");
       };
       int t = (int)it.t0;
+      unsigned nB = 0, nX = 0, nC = 0;  // loads issued
+      volatile int* abort_flag = &bar->abort;
 #pragma unroll 1
       for (unsigned c = 0; c < (unsigned)nblk; ++c, t += kQ) {
         const unsigned s = c & 1;
         if (c >= 2) wait(bar->emptyB[s], (c >> 1) - 1);
+        if (*abort_flag) break;
         mbar_arrive_expect_tx(&bar->fullB[s], p.nb * kBox);
 #pragma unroll 1
         for (int k = 0; k < p.nb; ++k) tma_tile(sm + kOffB + s * kTile + k * kBox, &p.mb, &bar->fullB[s], 64 * k, g, t, b);
+        ++nB;
         if (c >= 2) {
           if (PART)
             wait(bar->xF[s], (c >> 1) - 1);
           else
             store(c - 2);
         }
+        if (*abort_flag) break;
         mbar_arrive_expect_tx(&bar->fullX[s], kTile);
 #pragma unroll 1
         for (int k = 0; k < 2; ++k)
           tma_tile(sm + kOffX + s * kTile + k * kBox, &p.mx, &bar->fullX[s], WIDE ? 64 * k : 0, WIDE ? h0 : h0 + k, t, b);
+        ++nX;
         if (!PART) {
           if (c >= 1) wait(bar->emptyC, c - 1);
+          if (*abort_flag) break;
           mbar_arrive_expect_tx(&bar->fullC, p.nb * kBox);
 #pragma unroll 1
           for (int k = 0; k < p.nb; ++k) tma_tile(sm + kOffC + k * kBox, &p.mc, &bar->fullC, 64 * k, g, t, b);
+          ++nC;
         }
       }
       if (!PART) {
@@ -406,9 +482,9 @@ __global__ void __launch_bounds__(kThreads, 1) scan_tc_kernel(const __grid_const
         if (nblk > 0) store(nblk - 1);
       }
       // Nothing may land after the CTA has gone (normally all has landed).
-      mbar_drain(bar->fullB, nblk, 2);
-      mbar_drain(bar->fullX, nblk, 2);
-      if (!PART) mbar_drain(&bar->fullC, nblk, 1);
+      mbar_drain(bar->fullB, nB, 2);
+      mbar_drain(bar->fullX, nX, 2);
+      if (!PART) mbar_drain(&bar->fullC, nC, 1);
     }
   } else if (warp == 1) {
     // ---------------- products of y: G, inter, intra ----------------
@@ -493,7 +569,7 @@ __global__ void __launch_bounds__(kThreads, 1) scan_tc_kernel(const __grid_const
 #pragma unroll 1
       for (unsigned u = 0; u < 4; ++u) {
         const unsigned n = 4 * c + u;
-        wait(bar->wR[n & 1], n >> 1);
+        wait(bar->wR[u], c);
         tc_after();
         const uint64_t b = mB + ((s * kTile + u * 4096u) >> 4);
         uint32_t w = dW + (n & 1) * (16 * TERMS);
@@ -504,7 +580,7 @@ __global__ void __launch_bounds__(kThreads, 1) scan_tc_kernel(const __grid_const
             mma_ts(dD, w + 8, b + (2048u >> 4), id_st, 1);
           }
         }
-        if (lead) tc_commit(&bar->wF[n & 1]);
+        if (lead) tc_commit(&bar->wF[u]);
       }
       if (lead) {
         tc_commit(&bar->dR);
@@ -540,6 +616,7 @@ __global__ void __launch_bounds__(kThreads, 1) scan_tc_kernel(const __grid_const
       return d;
     };
     uint32_t raw = raw_step(0);
+    const Units<T, TERMS> units(sm, q, hf, lane);
     auto steps = [&](unsigned c) {
       if (cums) {
         Cum& u = cum[c & 1][hf];
@@ -561,6 +638,15 @@ __global__ void __launch_bounds__(kThreads, 1) scan_tc_kernel(const __grid_const
         u.u[row] = lane == 31 ? d : d * ex2_approx(r);
       }
       warp_arrive(&bar->cumF[c & 1]);
+      if (kShare) {
+        const unsigned s = c & 1;
+        wait(bar->cumF[s], c >> 1);
+        wait(bar->fullX[s], c >> 1);
+        if (a.cu != nullptr && it.t1 - it.t0 - (i64)c * kQ < kQ) wait(bar->xSync, 0);  // foreign rows are zeros
+        const Cum& u = cum[s][WIDE ? 0 : q >> 1];
+        const float one[4] = {1.f, 1.f, 1.f, 1.f};
+        units.make(bar, tmem + lanes, s, 4 * c, u.u, ex2_approx(u.tot[1] + (u.tot[2] + u.tot[3])), one);
+      }
     };
     if (PART) {
 #pragma unroll 1
@@ -776,7 +862,7 @@ __global__ void __launch_bounds__(kThreads, 1) scan_tc_kernel(const __grid_const
       }
     }
     float total = 0.f;   // base-2 log of the segment's decay
-    constexpr bool kRowScale = std::is_same<T, __half>::value;
+    const Units<T, TERMS> units(sm, q, hf, lane);
     float dec = 1.f, unscale = 1.f;
     // S = dec * S + dS of block c - 1 (c > 0), and with `copy` the 16-bit copy
     // of S for inter: row p, this thread's half of n.
@@ -824,19 +910,6 @@ __global__ void __launch_bounds__(kThreads, 1) scan_tc_kernel(const __grid_const
         warp_arrive(&bar->sR);
       }
     };
-    // x for w X comes transposed out of shared memory (ldmatrix), as lane l's
-    // columns p = l / 4 (+ 8, 16, 24) and tokens 2 (l % 4), + 1 of eight; the
-    // 16x128b stores put that into TMEM as rows p and columns of token pairs.
-    // Of each unit of 32 tokens this warp does 16: matrices of 8 tokens by 8
-    // columns in the order (first 8 tokens, second 8) x (8 columns, next 8).
-    const uint32_t xrow = smem_u32(sm) + kOffX + (q >> 1) * kBox + (16 * hf + ((lane >> 4) << 3) + (lane & 7)) * 128;
-    const uint32_t xcol0 = (((q & 1) * 4 + ((lane >> 3) & 1)) ^ (lane & 7)) << 4, xcol1 = xcol0 ^ (2 << 4);
-    const int wt = 16 * hf + 2 * (lane & 3);  // this lane's first token of a unit
-    auto load_x = [&](unsigned s, unsigned un, uint32_t (&x)[8]) {
-      const uint32_t at = xrow + s * kTile + un * (32 * 128);
-      ldmatrix_t(at + xcol0, x[0], x[1], x[2], x[3]);
-      ldmatrix_t(at + xcol1, x[4], x[5], x[6], x[7]);
-    };
 #pragma unroll 1
     for (unsigned c = 0; c < (unsigned)nblk; ++c) {
       const unsigned s = c & 1;
@@ -861,23 +934,22 @@ __global__ void __launch_bounds__(kThreads, 1) scan_tc_kernel(const __grid_const
       }
       wait(bar->cumF[s], c >> 1);
       const Cum& u = cum[s][hs];
-      const float* uw = u.u + wt;
       // Decay from the end of each sub-block to the block's end, of the whole block.
       const float after2 = u.tot[3], after1 = u.tot[2] + after2, after0 = u.tot[1] + after1;
       const float g0 = ex2_approx(after0), g1 = ex2_approx(after1), g2 = ex2_approx(after2);
-      uint32_t x[8];
       float scale[4] = {1.f, 1.f, 1.f, 1.f}, next_unscale = 1.f;
       const float next_dec = ex2_approx(u.tot[0] + after0);
-      if (kRowScale) {
+      if (kRowScale<T>) {
         // The largest |w x| of each row, of both its warps.
         float m[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
         for (unsigned un = 0; un < 4; ++un) {
-          load_x(s, un, x);
+          uint32_t x[8];
+          units.load(s, un, x);
           const float g = un == 0 ? g0 : un == 1 ? g1 : un == 2 ? g2 : 1.f;
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const float2 w = *reinterpret_cast<const float2*>(uw + 32 * un + 4 * (i & 2));
+            const float2 w = *reinterpret_cast<const float2*>(u.u + units.token + 32 * un + 4 * (i & 2));
             const float2 v = mul2(mul2(w, f2(g, g)), Pair<T>::unpack(x[i]));
             m[2 * (i >> 2) + (i & 1)] = fmaxf(m[2 * (i >> 2) + (i & 1)], fmaxf(fabsf(v.x), fabsf(v.y)));
           }
@@ -898,33 +970,11 @@ __global__ void __launch_bounds__(kThreads, 1) scan_tc_kernel(const __grid_const
         next_unscale = __uint_as_float((exponent(row) - 14u) << 23);
       }
 #pragma unroll 1
-      for (unsigned un = 0; un < 4; ++un) {
+      for (unsigned un = kShare ? 1 : 0; un < 4; ++un) {
         // The state of the block before, as soon as its last unit is through.
         if (un == 1) advance(c, !PART);
-        const unsigned n = 4 * c + un;
-        load_x(s, un, x);
         const float g = un == 0 ? g0 : un == 1 ? g1 : un == 2 ? g2 : 1.f;
-        const float2 w0 = mul2(*reinterpret_cast<const float2*>(uw + 32 * un), f2(g, g));
-        const float2 w1 = mul2(*reinterpret_cast<const float2*>(uw + 32 * un + 8), f2(g, g));
-        if (n >= 2) wait(bar->wF[n & 1], (n >> 1) - 1);
-        tc_after();
-        uint32_t o[TERMS][8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          float2 v = mul2((i & 2) ? w1 : w0, Pair<T>::unpack(x[i]));
-          if (kRowScale) v = mul2(v, f2(scale[2 * (i >> 2) + (i & 1)], scale[2 * (i >> 2) + (i & 1)]));
-#pragma unroll
-          for (int k = 0; k < TERMS; ++k) o[k][i] = take_term<T, (TERMS > 1)>(v);
-        }
-        const uint32_t at = tmem + lanes + kColW + (n & 1) * (16 * TERMS) + 8 * hf;
-#pragma unroll
-        for (int k = 0; k < TERMS; ++k) {
-          tm_st_16x128(at + 16 * k, o[k][0], o[k][1], o[k][2], o[k][3]);
-          tm_st_16x128(at + 16 * k + (16u << 16), o[k][4], o[k][5], o[k][6], o[k][7]);
-        }
-        tm_st_wait();
-        tc_before();
-        warp_arrive(&bar->wR[n & 1]);
+        units.make(bar, tmem + lanes, s, 4 * c + un, u.u, g, scale);
       }
       if (PART) total += u.tot[0] + after0;
       warp_arrive(&bar->xF[s]);  // x and the steps have been read
