@@ -401,6 +401,18 @@ def _pick(op, impl):
     return op if torch.compiler.is_compiling() else impl
 
 
+def _call(fn, p, x: torch.Tensor, what: str) -> None:
+    """fn(&p, the current stream of x's device) with that device current."""
+    dev = x.get_device()
+    if torch.cuda.current_device() == dev:
+        status = fn(ctypes.byref(p), torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with _on_device(x.device):
+            status = fn(ctypes.byref(p), torch._C._cuda_getCurrentRawStream(dev))
+    if status:
+        _lib.check(status, what)
+
+
 def _scan_impl(
     x: torch.Tensor,
     dt: torch.Tensor,
@@ -432,13 +444,14 @@ def _scan_impl(
         _ptr(init), *((0, 0) if init is None else init.stride()[:2]),
         y.data_ptr(), *y.stride()[:3],
         _ptr(final_states_out), *((0, 0) if final_states_out is None else final_states_out.stride()[:2]))
-    with _on_device(x.device):
-        n = ctypes.c_size_t(0)
-        _lib.check(lib.cc1d_scan_workspace_size(ctypes.byref(p), ctypes.byref(n)), "cc1d_scan_workspace_size")
-        if n.value > 0:
-            ws = torch.empty(n.value, dtype=torch.uint8, device=x.device)
-            p.workspace, p.workspace_bytes = ws.data_ptr(), n.value
-        _lib.check(lib.cc1d_scan(ctypes.byref(p), _stream(x.device)), "cc1d_scan")
+    n = ctypes.c_size_t(0)
+    status = lib.cc1d_scan_workspace_size(ctypes.byref(p), ctypes.byref(n))
+    if status:
+        _lib.check(status, "cc1d_scan_workspace_size")
+    if n.value > 0:
+        ws = torch.empty(n.value, dtype=torch.uint8, device=x.device)
+        p.workspace, p.workspace_bytes = ws.data_ptr(), n.value
+    _call(lib.cc1d_scan, p, x, "cc1d_scan")
 
 
 def _scan_fake(x, dt, A, B, C, D, dt_bias, dt_softplus, initial_states, cu_seqlens, max_seqlen, y,
@@ -478,8 +491,7 @@ def _scan_update_impl(
         x.data_ptr(), *x.stride(), dt.data_ptr(), *dt.stride(), B.data_ptr(), *B.stride(), C.data_ptr(), *C.stride(),
         A.data_ptr(), _ptr(D), _ptr(dt_bias), state.data_ptr(), *state.stride()[:3],
         _ptr(state_indices), _ptr(out_state_indices), y.data_ptr(), *y.stride()[:2])
-    with _on_device(x.device):
-        _lib.check(lib.cc1d_scan_update(ctypes.byref(p), _stream(x.device)), "cc1d_scan_update")
+    _call(lib.cc1d_scan_update, p, x, "cc1d_scan_update")
 
 
 def _scan_update_fake(x, state, dt, A, B, C, D, dt_bias, dt_softplus, state_indices, out_state_indices, y) -> None:
@@ -516,8 +528,7 @@ def _norm_fwd_impl(
         x.shape[0], x.shape[1], group_size, eps, 0,
         x.data_ptr(), x.stride(0), _ptr(z), 0 if z is None else z.stride(0), weight.data_ptr(), _ptr(bias),
         y.data_ptr(), y.stride(0), _ptr(mean), _ptr(rstd))
-    with _on_device(x.device):
-        _lib.check(lib.cc1d_gated_norm_fwd(ctypes.byref(p), _stream(x.device)), "cc1d_gated_norm_fwd")
+    _call(lib.cc1d_gated_norm_fwd, p, x, "cc1d_gated_norm_fwd")
 
 
 def _norm_fwd_fake(x, z, weight, bias, eps, group_size, layer, gate_first, y, mean, rstd) -> None:
@@ -558,13 +569,11 @@ def _norm_bwd_impl(
         x.data_ptr(), x.stride(0), _ptr(z), 0 if z is None else z.stride(0), weight.data_ptr(), _ptr(bias),
         0, 0, _ptr(mean), rstd.data_ptr(), dy.data_ptr(), dy.stride(0), dx.data_ptr(), dx.stride(0),
         _ptr(dz), 0 if dz is None else dz.stride(0), dweight.data_ptr(), _ptr(dbias))
-    with _on_device(x.device):
-        n = ctypes.c_size_t(0)
-        _lib.check(lib.cc1d_gated_norm_workspace_size(ctypes.byref(p), ctypes.byref(n)),
-                   "cc1d_gated_norm_workspace_size")
-        ws = torch.empty(n.value, dtype=torch.uint8, device=x.device)
-        p.workspace, p.workspace_bytes = ws.data_ptr(), n.value
-        _lib.check(lib.cc1d_gated_norm_bwd(ctypes.byref(p), _stream(x.device)), "cc1d_gated_norm_bwd")
+    n = ctypes.c_size_t(0)
+    _lib.check(lib.cc1d_gated_norm_workspace_size(ctypes.byref(p), ctypes.byref(n)), "cc1d_gated_norm_workspace_size")
+    ws = torch.empty(n.value, dtype=torch.uint8, device=x.device)
+    p.workspace, p.workspace_bytes = ws.data_ptr(), n.value
+    _call(lib.cc1d_gated_norm_bwd, p, x, "cc1d_gated_norm_bwd")
 
 
 def _norm_bwd_fake(x, z, weight, bias, dy, mean, rstd, eps, group_size, layer, gate_first, dx, dz, dweight,

@@ -47,17 +47,62 @@ __device__ __forceinline__ float reduce_rows(const float (&acc)[R], int i) {
 // any type, stride and size works.  Per token and state value: one multiply,
 // two fused multiply-adds.  Taken for fp32 data (the tensor cores would round
 // it), for shapes the tensor-core kernel does not take, and for short calls.
-constexpr int kWalkTokens = 16;
+// Bound by the fp32 pipe on wide states: 1.5 packed instructions per value.
 constexpr int kWalkThreads = 128;
+// Tokens per staged chunk: as many as 48 KB of shared memory hold twice.
+constexpr int walk_tokens(int np) { return np >= 256 ? 8 : np >= 64 ? 16 : 32; }
+
+// 16 bytes from global to shared memory without registers, or zeros.
+__device__ __forceinline__ void copy16(void* dst, const void* src, bool ok) {
+  const unsigned d = static_cast<unsigned>(__cvta_generic_to_shared(dst)), n = ok ? 16u : 0u;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(src), "r"(n) : "memory");
+}
+
+// Rows [0, TOK) of a (tokens, n) operand into fp32 shared memory, zeros
+// outside nt x n.  Of unit stride and 16-byte aligned rows, 16 bytes at a time
+// (fp32: asynchronously, for the next wait_group); else element by element.
+template <typename T, int TOK, int NP>
+__device__ __forceinline__ void stage_rows(float (&to)[TOK][NP], const T* p, i64 ts, i64 ns, int nt, int n, bool wide) {
+  constexpr int V = 16 / (int)sizeof(T);
+  if (wide && NP % V == 0) {
+    constexpr int W = NP >= V ? NP / V : 1;
+    for (int e = threadIdx.x; e < TOK * W; e += kWalkThreads) {
+      const int t = e / W, c = (e % W) * V;
+      const bool ok = t < nt && c < n;
+      const T* src = p + (ok ? t * ts + c : 0);
+      if constexpr (sizeof(T) == 4) {
+        copy16(&to[t][c], src, ok);
+      } else {
+        Pack<T, V> pk;
+        if (ok) pk = ld_pack<T, V>(src);
+#pragma unroll
+        for (int j = 0; j < V; ++j) to[t][c + j] = ok ? Cvt<T>::f(pk.v[j]) : 0.f;
+      }
+    }
+  } else {
+    for (int e = threadIdx.x; e < TOK * NP; e += kWalkThreads) {
+      const int t = e / NP, c = e % NP;
+      to[t][c] = t < nt && c < n ? Cvt<T>::f(p[t * ts + c * ns]) : 0.f;
+    }
+  }
+}
+
+// Whether rows of n values can be read 16 bytes at a time.
+template <typename T>
+__device__ __forceinline__ bool wide_rows(const T* p, i64 ts, i64 ns, int n) {
+  constexpr int V = 16 / (int)sizeof(T);
+  return ns == 1 && n % V == 0 && ts % V == 0 && reinterpret_cast<uintptr_t>(p) % 16 == 0;
+}
 
 template <typename T, int VEC, int NV, int R, bool PART>
 __global__ void __launch_bounds__(kWalkThreads) scan_walk_kernel(const __grid_constant__ ScanArgs a) {
   constexpr int NP = 8 * VEC * NV;   // padded state size
   constexpr int ROWS = 16 * R;       // rows per block
-  __shared__ __align__(16) float sB[kWalkTokens][NP];
-  __shared__ __align__(16) float sC[PART ? 1 : kWalkTokens][NP];
-  __shared__ float sx[kWalkTokens][ROWS];
-  __shared__ float sa[kWalkTokens], sd[kWalkTokens];
+  constexpr int kWalkTokens = walk_tokens(NP);
+  __shared__ __align__(16) float sB[2][kWalkTokens][NP];
+  __shared__ __align__(16) float sC[2][PART ? 1 : kWalkTokens][NP];
+  __shared__ __align__(16) float sx[2][kWalkTokens][ROWS];
+  __shared__ float sa[2][kWalkTokens], sd[2][kWalkTokens];
   griddep_wait();
   const int h = blockIdx.x % a.H;
   const i64 item = blockIdx.x / a.H;
@@ -68,6 +113,7 @@ __global__ void __launch_bounds__(kWalkThreads) scan_walk_kernel(const __grid_co
   const int row_b = blockIdx.y * ROWS;                     // first row of the block
   const int row_w = warp * 4 * R + (lane >> 3) * R;        // this lane group's first row within it
   const int g = h / a.R;
+  auto state_at = [&](int v) { return ((v / VEC) * 8 + i) * VEC + v % VEC; };  // this lane's v-th state value
   const float A2 = a.A[h] * kLog2e;
   const float bias = a.dt_bias ? a.dt_bias[h] : 0.f;
   const float Dh = a.D ? a.D[h] : 0.f;
@@ -77,13 +123,13 @@ __global__ void __launch_bounds__(kWalkThreads) scan_walk_kernel(const __grid_co
   const i64 dto = it.batch * a.ds_b + h * a.ds_h;
   T* y = static_cast<T*>(a.y) + it.batch * a.ys_b + h * a.ys_h;
 
-  float S[R][NV * VEC];
+  float2 S[R][NV * VEC / 2];  // pairs along the state size: packed fp32 math
 #pragma unroll
   for (int k = 0; k < R; ++k) {
     const int row = row_b + row_w + k;
 #pragma unroll
     for (int v = 0; v < NV * VEC; ++v) {
-      const int n = ((v / VEC) * 8 + i) * VEC + v % VEC;
+      const int n = state_at(v);
       float s = 0.f;
       if (!PART && row < a.P && n < a.N) {
         const i64 e = (i64)row * a.N + n;
@@ -96,65 +142,88 @@ __global__ void __launch_bounds__(kWalkThreads) scan_walk_kernel(const __grid_co
           s = fmaf(s, ex2_approx(a.decay[slot]), a.part[slot * a.P * a.N + e]);
         }
       }
-      S[k][v] = s;
+      if (v % 2)
+        S[k][v / 2].y = s;
+      else
+        S[k][v / 2].x = s;
     }
   }
   float total = 0.f;  // log2 of the segment's decay
-  for (i64 t0 = it.t0; t0 < it.t1; t0 += kWalkTokens) {
+  const bool wideB = wide_rows(Bp, a.bs_t, a.bs_n, a.N), wideC = wide_rows(Cp, a.cs_t, a.cs_n, a.N);
+  const int rows = min(a.P - row_b, ROWS);
+  const bool widex = wide_rows(x + row_b * a.xs_p, a.xs_t, a.xs_p, rows);
+  // dt of this thread's token of a chunk, asked for a chunk ahead.
+  auto raw_step = [&](i64 t0) {
+    return tid < kWalkTokens && t0 + tid < it.t1 ? scan_raw_step<T>(a, dto + (t0 + tid) * a.ds_t) : 0.f;
+  };
+  float raw = raw_step(it.t0);
+  auto stage = [&](int buf, i64 t0) {
     const int nt = (int)min((i64)kWalkTokens, it.t1 - t0);
-    __syncthreads();
-    for (int e = tid; e < kWalkTokens * NP; e += kWalkThreads) {
-      const int t = e / NP, n = e % NP;
-      const bool ok = t < nt && n < a.N;
-      sB[t][n] = ok ? Cvt<T>::f(Bp[(t0 + t) * a.bs_t + n * a.bs_n]) : 0.f;
-      if (!PART) sC[t][n] = ok ? Cvt<T>::f(Cp[(t0 + t) * a.cs_t + n * a.cs_n]) : 0.f;
-    }
-    for (int e = tid; e < kWalkTokens * ROWS; e += kWalkThreads) {
-      const int t = e / ROWS, r = e % ROWS;
-      sx[t][r] = t < nt && row_b + r < a.P ? Cvt<T>::f(x[(t0 + t) * a.xs_t + (row_b + r) * a.xs_p]) : 0.f;
-    }
+    stage_rows<T>(sB[buf], Bp + t0 * a.bs_t, a.bs_t, a.bs_n, nt, a.N, wideB);
+    if constexpr (!PART) stage_rows<T>(sC[buf], Cp + t0 * a.cs_t, a.cs_t, a.cs_n, nt, a.N, wideC);
+    stage_rows<T>(sx[buf], x + t0 * a.xs_t + row_b * a.xs_p, a.xs_t, a.xs_p, nt, rows, widex);
+    asm volatile("cp.async.commit_group;" ::: "memory");
     if (tid < nt) {
-      const float d = scan_step<T>(a, dto + (t0 + tid) * a.ds_t, bias);
-      sd[tid] = d;
-      sa[tid] = d * A2;
+      const float v = raw + bias, d = a.softplus ? softplus_f(v) : v;
+      sd[buf][tid] = d;
+      sa[buf][tid] = d * A2;
+    }
+    raw = raw_step(t0 + kWalkTokens);
+  };
+  if (it.t0 < it.t1) stage(0, it.t0);
+  int buf = 0;
+  for (i64 t0 = it.t0; t0 < it.t1; t0 += kWalkTokens, buf ^= 1) {
+    const int nt = (int)min((i64)kWalkTokens, it.t1 - t0);
+    // The next chunk is on its way while this one is worked on.
+    if (t0 + kWalkTokens < it.t1) {
+      stage(buf ^ 1, t0 + kWalkTokens);
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
+    } else {
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
     }
     __syncthreads();
 #pragma unroll 2
     for (int t = 0; t < nt; ++t) {
-      const float d = sd[t], l = sa[t], w = ex2_approx(l);
+      const float d = sd[buf][t], l = sa[buf][t], w = ex2_approx(l);
       if (PART) total += l;
-      float u[R], acc[R];
+      const float2 ww = f2(w, w);
+      float2 u[R], sum[R];
 #pragma unroll
       for (int k = 0; k < R; ++k) {
-        u[k] = d * sx[t][row_w + k];
-        acc[k] = 0.f;
+        const float ux = d * sx[buf][t][row_w + k];
+        u[k] = f2(ux, ux);
+        sum[k] = f2(0.f, 0.f);
       }
 #pragma unroll
       for (int v = 0; v < NV; ++v) {
-        float b[VEC], c[VEC];
+        float2 b[VEC / 2], c[VEC / 2];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) b[j] = sB[t][(v * 8 + i) * VEC + j];
+        for (int j = 0; j < VEC / 2; ++j) b[j] = *reinterpret_cast<const float2*>(&sB[buf][t][(v * 8 + i) * VEC + 2 * j]);
         if (!PART) {
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) c[j] = sC[t][(v * 8 + i) * VEC + j];
+          for (int j = 0; j < VEC / 2; ++j) c[j] = *reinterpret_cast<const float2*>(&sC[buf][t][(v * 8 + i) * VEC + 2 * j]);
         }
 #pragma unroll
         for (int k = 0; k < R; ++k) {
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            float& s = S[k][v * VEC + j];
-            s = fmaf(s, w, u[k] * b[j]);
-            if (!PART) acc[k] = fmaf(s, c[j], acc[k]);
+          for (int j = 0; j < VEC / 2; ++j) {
+            float2& s = S[k][v * VEC / 2 + j];
+            s = fma2(s, ww, mul2(u[k], b[j]));
+            if (!PART) sum[k] = fma2(s, c[j], sum[k]);
           }
         }
       }
       if (!PART) {
+        float acc[R];
+#pragma unroll
+        for (int k = 0; k < R; ++k) acc[k] = sum[k].x + sum[k].y;
         const float v = reduce_rows<R>(acc, i);
         const int r = row_w + i / (8 / R);
         if ((i & (8 / R - 1)) == 0 && row_b + r < a.P)
-          y[(t0 + t) * a.ys_t + row_b + r] = Cvt<T>::to(fmaf(Dh, sx[t][r], v));
+          y[(t0 + t) * a.ys_t + row_b + r] = Cvt<T>::to(fmaf(Dh, sx[buf][t][r], v));
       }
     }
+    __syncthreads();
   }
   float* out = nullptr;
   if (PART) {
@@ -170,8 +239,8 @@ __global__ void __launch_bounds__(kWalkThreads) scan_walk_kernel(const __grid_co
     const int row = row_b + row_w + k;
 #pragma unroll
     for (int v = 0; v < NV * VEC; ++v) {
-      const int n = ((v / VEC) * 8 + i) * VEC + v % VEC;
-      if (row < a.P && n < a.N) out[(i64)row * a.N + n] = S[k][v];
+      const int n = state_at(v);
+      if (row < a.P && n < a.N) out[(i64)row * a.N + n] = v % 2 ? S[k][v / 2].y : S[k][v / 2].x;
     }
   }
 }
@@ -221,9 +290,11 @@ cudaError_t launch_walk(const ScanArgs& a, bool split, cudaStream_t stream) {
 // ---- one token per row, the state in memory ----
 //
 // Bound by the state's bytes (read once, written once); the rest is a few
-// hundred values per head.  Eight lanes share a state row, as above, with
-// VEC values (16 bytes where the layout allows) per access; a thread issues
-// the loads of all its R rows before it uses one.
+// hundred values per head.  Eight lanes share a state row, as above, with VEC
+// values (16 bytes where the layout allows) per access; a thread issues the
+// loads of all its R rows before it uses one, and loads and stores are marked
+// evict-first.  256 rows of 80 heads of 64 x 128 in fp32: 219 us, 6.1 TB/s;
+// with ordinary accesses 239, with 4 rows per thread 250, with one 265.
 struct UpdArgs {
   const void* x; i64 xs_b, xs_h, xs_p;
   const void* dt; i64 ds_b, ds_h;
@@ -270,7 +341,7 @@ __global__ void __launch_bounds__(128) scan_update_kernel(const __grid_constant_
     for (int v = 0; v < NV; ++v) {
       const int n = (v * 8 + i) * VEC;
       if (row0 + k < a.P && n < a.N)
-        s[k][v].raw = *reinterpret_cast<const typename Pack<ST, VEC>::Raw*>(sp + (row0 + k) * a.ss_p + n);
+        s[k][v].raw = __ldcs(reinterpret_cast<const typename Pack<ST, VEC>::Raw*>(sp + (row0 + k) * a.ss_p + n));
       else
         s[k][v].raw = typename Pack<ST, VEC>::Raw();
     }
@@ -309,7 +380,7 @@ __global__ void __launch_bounds__(128) scan_update_kernel(const __grid_constant_
         o.v[j] = Cvt<ST>::to(t);
       }
       if (keep && row0 + k < a.P && n < a.N)
-        *reinterpret_cast<typename Pack<ST, VEC>::Raw*>(dp + (row0 + k) * a.ss_p + n) = o.raw;
+        __stcs(reinterpret_cast<typename Pack<ST, VEC>::Raw*>(dp + (row0 + k) * a.ss_p + n), o.raw);
     }
   }
   const float v = reduce_rows<R>(acc, i);
@@ -322,7 +393,7 @@ __global__ void __launch_bounds__(128) scan_update_kernel(const __grid_constant_
 
 template <typename T, typename ST, int VEC, int NV>
 cudaError_t launch_upd_n(const UpdArgs& a, i64 batch, cudaStream_t stream) {
-  constexpr int R = NV * VEC <= 16 ? 4 : NV * VEC <= 32 ? 2 : 1;
+  constexpr int R = NV * VEC <= 32 ? 2 : 1;
   if (a.P > 16 && batch * a.H * ceil_div(a.P, 16 * R) >= 1024) {
     const dim3 grid((unsigned)(batch * a.H), (unsigned)ceil_div(a.P, 16 * R));
     return launch_pdl(scan_update_kernel<T, ST, VEC, NV, R>, grid, dim3(128), 0, stream, a);
