@@ -111,8 +111,9 @@ def state_space_scan(
     final_states (num_seqs, nheads, headdim, dstate) in float32.
 
     bf16 and fp16 prompts run on the tensor cores; the state is kept in fp32 between
-    blocks of tokens.  There a non-finite x, B or C can reach earlier tokens of its own
-    sequence within its block of 128 tokens (not other sequences).
+    blocks of tokens.  There a non-finite x, B, C or dt can reach earlier tokens of its own
+    sequence within its block of 128 tokens (not other sequences), and fp16 state values
+    beyond 65504 overflow in y (not in the state).
     """
     if x.dim() != 4 or dt.dim() != 3 or B.dim() != 4 or C.dim() != 4:
         raise ValueError("x must be (batch, seqlen, nheads, headdim), dt (batch, seqlen, nheads), "

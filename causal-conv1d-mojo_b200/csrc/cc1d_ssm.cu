@@ -475,7 +475,8 @@ int plan_scan(const cc1d_scan_params* p, ScanArgs* a, ScanPlan* plan) {
                 (nseq == 0 ? (p->batch == 0 || p->seqlen == 0 || p->cu_seqlens == nullptr)
                            : (p->seqlen == 0 && p->final_states == nullptr));
   if (plan->empty) return CC1D_OK;
-  if (nseq > 0x7fffff || p->seqlen > 0x7fffffffLL)
+  // Token counts and the launch's blocks (a segment has 64 tokens or more) fit 31 bits.
+  if (p->seqlen > 0x7fffffffLL - 65536 || (nseq + (nseq > 0 ? p->seqlen / 64 : 0)) * p->nheads > 0x7fffffffLL)
     return report_error(CC1D_ERR_UNSUPPORTED, "cc1d_scan: too many sequences or tokens");
   if ((p->seqlen > 0 && (!p->x || !p->dt || !p->y || (p->dstate > 0 && (!p->B || !p->C)))) || !p->A)
     return report_error(CC1D_ERR_INVALID_ARGUMENT, "cc1d_scan: x, dt, A, B, C and y are required");
