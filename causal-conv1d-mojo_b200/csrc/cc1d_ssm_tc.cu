@@ -44,17 +44,26 @@
 //   warp 2       issues dS: the chains of y and of the state meet only where
 //                one needs the other, and one issuer for both would make each
 //                wait for the other's barriers
-//   warps 4-11   tokens: thread = token row.  Steps, decays and the first unit of
-//                (w X)^T of the next block;  M from G, in place in TMEM (16
-//                fp32 columns become 8 + 8 of pairs, one head each); scales inter by exp(c_i), so that intra accumulates
-//                onto it; y + D x over x in shared memory
+//   warps 4-11   tokens: thread = token row.  Steps, decays and (bf16) the first
+//                unit of (w X)^T of the next block;  M from G, in place in
+//                TMEM (16 fp32 columns become 8 + 8 of pairs, one head each);
+//                scales inter by exp(c_i), so that intra accumulates onto it;
+//                y + D x over x in shared memory
 //   warps 12-19  state: thread = row p of S, half of n.  (w X)^T into TMEM,
 //                S = exp(c_Q) S + dS, 16-bit copy to shared memory
 // TMEM (512 columns): G / M 128, y 128, dS 128, (w X)^T two buffers of one
-// unit (32 tokens, 16 columns a term).  (w X)^T comes from TMEM and not from shared memory because
-// the products' operands already take most of the shared-memory bandwidth.
+// unit (32 tokens, 16 columns a term).  (w X)^T comes from TMEM and not from
+// shared memory because the products' operands already take most of the
+// shared-memory bandwidth.
 // What a role does between two waits is kept short: with few warps it runs at
 // the latency of its instructions.
+//
+// Measured: 8 x 2048 tokens of 80 heads of 64 x 128, bf16 with final states,
+// 182 us (2.0 TB/s of data; the token-by-token walk takes 2999); one prompt
+// of 16384, cut into segments, 291; 65536 packed fp16 tokens of 60 heads 556.
+// Bound by the instructions of the 16 warps that feed the products, not by
+// these or by memory: issue slots 53-61 % busy, the tensor pipe 35-39 %, DRAM under
+// a third.
 //
 // A barrier tells only two phases apart: a waiter has to know that the phase
 // before the one it waits for is over, and the one after must not end before
