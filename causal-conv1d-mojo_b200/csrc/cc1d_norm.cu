@@ -14,7 +14,8 @@
 // read once per team and their gradients' sums stay in registers.
 // Measured on 16384 rows of 5120 in bf16, gated: forward 91 us (5.5 TB/s, 86 %
 // of a plain copy's rate), backward 185 (4.5 TB/s; two passes over a row, each
-// with SiLU: issue slots 62 % busy).  A single row: 1.8 us.
+// with SiLU: issue slots 62 % busy).  A single row: 3.0 us,
+// in groups of 640 2.1.
 #include <algorithm>
 #include <cstring>
 
@@ -832,13 +833,16 @@ int plan_norm(const char* what, const cc1d_gated_norm_params* p, bool bwd, NormA
     const int resident = std::max(1, 1024 / plan->threads);
     const unsigned stage = (unsigned)(a->gs * es) * ((bwd ? 2 : 1) + (p->z ? 1 : 0));
     if (!plan->warp_teams && vec) {
-      // A ring when rows per block are many, of 2 to 4 stages in what shared
-      // memory the resident blocks have.
+      // A ring where every resident block has a row, of 2 to 4 stages in what
+      // shared memory these have.  Rows of 5120 in bf16, gated (ring | registers,
+      // us): 148 rows 3.8 | 3.4, 444 rows 5.4 | 6.1, 1776 rows 12 | 16, 16384
+      // rows 92 | 223; forward and backward 148 rows 14.0 | 12.7, 444 rows
+      // 25 | 27, 16384 rows 271 | 626.
       const i64 fill = ceil_div((i64)sms * resident, a->groups);
       const int room = 220 * 1024 / resident;
       const int params = a->gs * (a->w_f32 ? 4 : es) * (p->bias ? 2 : 1);
       const int stages = std::min(4, (int)((room - 1024 - params) / (int)stage));
-      if (stages >= 2 && p->rows >= 4 * fill) plan->stages = stages;
+      if (stages >= 2 && p->rows >= fill) plan->stages = stages;
     }
     const i64 fill = ceil_div((i64)sms * resident, a->groups);
     plan->blocks = std::max<i64>(1, std::min<i64>(ceil_div(p->rows, per_block), fill));

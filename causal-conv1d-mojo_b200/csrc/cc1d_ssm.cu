@@ -46,7 +46,7 @@ __device__ __forceinline__ float reduce_rows(const float (&acc)[R], int i) {
 // tokens that is staged in shared memory as fp32 (B, C, x, decay, step), so
 // any type, stride and size works.  Per token and state value: one multiply,
 // two fused multiply-adds.  Taken for fp32 data (the tensor cores would round
-// it), for shapes the tensor-core kernel does not take, and for short calls.
+// it), for shapes the tensor-core kernel does not take, and for short sequences.
 // Bound by the fp32 pipe on wide states (1.5 packed instructions per value)
 // and the latency of a token's sums: 8 x 1024 fp32 tokens of 80 heads of
 // 64 x 128 take 1011 us (1342 with scalar math and one chunk in flight);
@@ -296,8 +296,9 @@ cudaError_t launch_walk(const ScanArgs& a, bool split, cudaStream_t stream) {
 // hundred values per head.  Eight lanes share a state row, as above, with VEC
 // values (16 bytes where the layout allows) per access; a thread issues the
 // loads of all its R rows before it uses one, and loads and stores are marked
-// evict-first.  256 rows of 80 heads of 64 x 128 in fp32: 219 us, 6.1 TB/s;
-// with ordinary accesses 239, with 4 rows per thread 250, with one 265.
+// evict-first.  256 rows of 80 heads of 64 x 128 in fp32: 213 us, 6.3 TB/s;
+// with ordinary accesses 239, with 4 rows per thread 250, with one 259.  Two
+// are also sooner on few blocks (one row 3.9 | 4.0 us, 8 rows 8.1 | 10.4).
 struct UpdArgs {
   const void* x; i64 xs_b, xs_h, xs_p;
   const void* dt; i64 ds_b, ds_h;
@@ -397,11 +398,11 @@ __global__ void __launch_bounds__(128) scan_update_kernel(const __grid_constant_
 template <typename T, typename ST, int VEC, int NV>
 cudaError_t launch_upd_n(const UpdArgs& a, i64 batch, cudaStream_t stream) {
   constexpr int R = NV * VEC <= 32 ? 2 : 1;
-  if (a.P > 16 && batch * a.H * ceil_div(a.P, 16 * R) >= 1024) {
+  if (a.P > 16) {
     const dim3 grid((unsigned)(batch * a.H), (unsigned)ceil_div(a.P, 16 * R));
     return launch_pdl(scan_update_kernel<T, ST, VEC, NV, R>, grid, dim3(128), 0, stream, a);
   }
-  // Few rows: one state row per lane group, so that more SMs take part.
+  // A head of 16 rows or fewer: one state row per lane group uses all of them.
   const dim3 grid((unsigned)(batch * a.H), (unsigned)ceil_div(a.P, 16));
   return launch_pdl(scan_update_kernel<T, ST, VEC, NV, 1>, grid, dim3(128), 0, stream, a);
 }
@@ -499,10 +500,17 @@ int plan_scan(const cc1d_scan_params* p, ScanArgs* a, ScanPlan* plan) {
   a->segs = 1;
   a->items = nseq;
   if (nseq == 0 || p->seqlen == 0) return CC1D_OK;
-  // The tensor cores work in blocks of 128 tokens: below 16 tokens a sequence
-  // the walk over tokens is done sooner.
+  // The tensor cores take a block of 128 tokens' time for any part of one, the
+  // walk its tokens' and its state's.  Where they meet, by measurement (tensor
+  // cores | walk, us; 2560 rows of sequence and head, 16-bit data):
+  //   64 x 128, 5120 rows   1 token 236 | 371, 16 tokens 238 | 419
+  //   64 x 64               1 token 86 | 45, 16 tokens 88 | 70, 64 tokens 92 | 179
+  //   64 x 32               16 tokens 78 | 38, 64 tokens 81 | 99
+  //   16 x 64               16 tokens 73 | 29, 64 tokens 74 | 89
+  // and with few rows (96 of 64 x 64, 16 tokens 10.6 | 11.3) somewhat earlier.
   const i64 mean = p->cu_seqlens ? ceil_div(p->seqlen, nseq) : p->seqlen;
-  plan->tc = mean >= 16 && scan_tc_eligible(p->dtype, *a, p->batch);
+  const bool enough = (a->P >= 64 && a->N > 64) || mean >= 48 || mean * a->P * a->N >= 65536;
+  plan->tc = enough && scan_tc_eligible(p->dtype, *a, p->batch);
   DeviceInfo dev;
   const cudaError_t de = device_info(&dev);
   const i64 sms = de == cudaSuccess ? dev.sms : 148;
