@@ -49,8 +49,8 @@ __device__ __forceinline__ float reduce_rows(const float (&acc)[R], int i) {
 // it), for shapes the tensor-core kernel does not take, and for short sequences.
 // Bound by the fp32 pipe on wide states (1.5 packed instructions per value)
 // and the latency of a token's sums: 8 x 1024 fp32 tokens of 80 heads of
-// 64 x 128 take 1011 us (1342 with scalar math and one chunk in flight);
-// 2 x 512 of 4 heads of 16 x 16 take 15, in segments.
+// 64 x 128 take 1001 us (1342 with scalar math and one chunk in flight);
+// 2 x 512 of 4 heads of 16 x 16 take 14.5, in segments.
 constexpr int kWalkThreads = 128;
 // Tokens per staged chunk: as many as 48 KB of shared memory hold twice.
 constexpr int walk_tokens(int np) { return np >= 256 ? 8 : np >= 64 ? 16 : 32; }
@@ -105,7 +105,8 @@ __global__ void __launch_bounds__(kWalkThreads) scan_walk_kernel(const __grid_co
   __shared__ __align__(16) float sB[2][kWalkTokens][NP];
   __shared__ __align__(16) float sC[2][PART ? 1 : kWalkTokens][NP];
   __shared__ __align__(16) float sx[2][kWalkTokens][ROWS];
-  __shared__ float sa[2][kWalkTokens], sd[2][kWalkTokens];
+  __shared__ float sw[2][kWalkTokens], sd[2][kWalkTokens];  // decay and step
+  __shared__ float sl[2][PART ? kWalkTokens : 1];           // log of the decay
   griddep_wait();
   const int h = blockIdx.x % a.H;
   const i64 item = blockIdx.x / a.H;
@@ -117,7 +118,7 @@ __global__ void __launch_bounds__(kWalkThreads) scan_walk_kernel(const __grid_co
   const int row_w = warp * 4 * R + (lane >> 3) * R;        // this lane group's first row within it
   const int g = h / a.R;
   auto state_at = [&](int v) { return ((v / VEC) * 8 + i) * VEC + v % VEC; };  // this lane's v-th state value
-  const float A2 = a.A[h] * kLog2e;
+  const float A = a.A[h];
   const float bias = a.dt_bias ? a.dt_bias[h] : 0.f;
   const float Dh = a.D ? a.D[h] : 0.f;
   const T* x = static_cast<const T*>(a.x) + it.batch * a.xs_b + h * a.xs_h;
@@ -142,7 +143,7 @@ __global__ void __launch_bounds__(kWalkThreads) scan_walk_kernel(const __grid_co
         }
         for (int r = 0; r < it.seg; ++r) {  // the earlier segments, in order
           const i64 slot = (it.first + r) * a.H + h;
-          s = fmaf(s, ex2_approx(a.decay[slot]), a.part[slot * a.P * a.N + e]);
+          s = fmaf(s, expf(a.decay[slot]), a.part[slot * a.P * a.N + e]);
         }
       }
       if (v % 2)
@@ -151,7 +152,7 @@ __global__ void __launch_bounds__(kWalkThreads) scan_walk_kernel(const __grid_co
         S[k][v / 2].x = s;
     }
   }
-  float total = 0.f;  // log2 of the segment's decay
+  float total = 0.f;  // log of the segment's decay
   const bool wideB = wide_rows(Bp, a.bs_t, a.bs_n, a.N), wideC = wide_rows(Cp, a.cs_t, a.cs_n, a.N);
   const int rows = min(a.P - row_b, ROWS);
   const bool widex = wide_rows(x + row_b * a.xs_p, a.xs_t, a.xs_p, rows);
@@ -169,7 +170,11 @@ __global__ void __launch_bounds__(kWalkThreads) scan_walk_kernel(const __grid_co
     if (tid < nt) {
       const float v = raw + bias, d = a.softplus ? softplus_f(v) : v;
       sd[buf][tid] = d;
-      sa[buf][tid] = d * A2;
+      // Accurate to the last bit or two: a state multiplies hundreds of these,
+      // and the error of an approximate exponential (always to one side for one
+      // step length) would add up to several times the rounding of fp32.
+      sw[buf][tid] = expf(d * A);
+      if (PART) sl[buf][tid] = d * A;
     }
     raw = raw_step(t0 + kWalkTokens);
   };
@@ -187,8 +192,8 @@ __global__ void __launch_bounds__(kWalkThreads) scan_walk_kernel(const __grid_co
     __syncthreads();
 #pragma unroll 2
     for (int t = 0; t < nt; ++t) {
-      const float d = sd[buf][t], l = sa[buf][t], w = ex2_approx(l);
-      if (PART) total += l;
+      const float d = sd[buf][t], w = sw[buf][t];
+      if (PART) total += sl[buf][t];
       const float2 ww = f2(w, w);
       float2 u[R], sum[R];
 #pragma unroll
@@ -354,7 +359,7 @@ __global__ void __launch_bounds__(128) scan_update_kernel(const __grid_constant_
   float d = a.dt_f32 ? static_cast<const float*>(a.dt)[dto] : Cvt<T>::f(static_cast<const T*>(a.dt)[dto]);
   if (a.dt_bias) d += a.dt_bias[h];
   if (a.softplus) d = softplus_f(d);
-  const float w = ex2_approx(d * (a.A[h] * kLog2e));
+  const float w = expf(d * a.A[h]);  // accurate: a decode multiplies thousands of these
   const float Dh = a.D ? a.D[h] : 0.f;
   float u[R], xr[R], acc[R];
 #pragma unroll

@@ -29,7 +29,7 @@ struct ScanArgs {
   void* y; i64 ys_b, ys_t, ys_h;
   float* fin; i64 fs_s, fs_h;
   float* part;         // [segments][heads][P][N]: a segment's state from zero
-  float* decay;        // [segments][heads]: log2 of its decay
+  float* decay;        // [segments][heads]: log of its decay (natural in the walk, base 2 on the tensor cores)
   i64 L;               // tokens of a row
   int H, P, N, G, R;   // R = H / G heads per group
   int nseq;
